@@ -8,3 +8,4 @@ from .index import (  # noqa: F401
     COSINE, EUCLIDEAN, L2_SQUARED, MAX_AGGREGATION, MEAN_AGGREGATION, SUM_AGGREGATION, Context, FlatIndex, IVFIndex,
     IVFPQIndex, PQIndex, HNSWIndex, BM25SearchIndex, SegmentSet, TextResult, TextSearch, UnknownDistanceKind, VectorIndex, VectorResult, VectorSearch, aggregate, autocut, sanitize_k,
 )
+from .rows import Fp8Rows, Fp8SearchResult, LogProbs  # noqa: F401

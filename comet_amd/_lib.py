@@ -21,6 +21,7 @@ ERR_ALREADY_DELETED, ERR_TRAIN_DATA, ERR_HIP, ERR_NO_DEVICE, ERR_UNSUPPORTED, ER
 ERR_FORMAT, ERR_IO = 12, 13
 
 L2, L2SQ, COSINE = 0, 1, 2
+F32, F16, BF16 = 0, 1, 2
 KIND_FLAT, KIND_IVF, KIND_PQ, KIND_IVFPQ, KIND_HNSW, KIND_BM25 = range(6)
 
 
@@ -159,12 +160,23 @@ def load() -> C.CDLL:
         "comet_index_serialize": (i32, [p, p, sz, C.POINTER(sz)]),
         "comet_index_deserialize": (i32, [p, p, sz, C.POINTER(sz)]),
         "comet_index_get_stat": (i32, [p, C.c_char_p, C.POINTER(C.c_double)]),
+        "comet_fp8_create": (i32, [p, i64, i32, pp]),
+        "comet_fp8_destroy": (i32, [p]),
+        "comet_fp8_capacity": (i64, [p]),
+        "comet_fp8_dim": (i32, [p]),
+        "comet_fp8_write_dev": (i32, [p, p, i64, p, i32, i64, i64, p]),
+        "comet_fp8_read_dev": (i32, [p, p, i64, p, i32, i64, i64, p]),
+        "comet_fp8_write": (i32, [p, p, p, i64]),
+        "comet_fp8_read": (i32, [p, p, i64, p]),
+        "comet_fp8_scores_dev": (i32, [p, i64, i64, p, i64, i64, p, i32, i64, p]),
+        "comet_logprobs_work_bytes": (i32, [i64, i64, i32, C.POINTER(sz)]),
+        "comet_logprobs_dev": (i32, [p, p, i32, i64, i64, i64, p, f32, p, i32, i32, p, p, p, p, p, p, sz, p]),
+        "comet_fp8_search": (i32, [p, i64, i64, p, i32, f32, i32, p, p, p, p]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(lib, name)  # AttributeError if the library lacks a declared symbol
         fn.restype = res
         fn.argtypes = args
-    _ = f32
     _lib = lib
     return lib
 

@@ -375,6 +375,58 @@ COMET_API int comet_index_export(const comet_index* idx, uint32_t* out_ids, int3
  * "fast_expansions", "fast_queries", "strict_queries", "max_abs", "max_norm2". Unknown name -> INVALID_ARG. */
 COMET_API int comet_index_get_stat(const comet_index* idx, const char* name, double* out);
 
+/* ---- rows in 8-bit floating point --------------------------------------------------------------------
+ * A store of `capacity` slots, each holding one row of `dim` numbers as e4m3 codes with a power-of-two scale per block of 128 consecutive
+ * numbers (the last block padded with zeros): 1.01 bytes a number instead of 4, no training, any slot rewritten at any time. The reference's
+ * nearest relative is its Int8Quantizer (quantizer.go; not used by any of its indexes); scores here are approximate where the indexes' are exact.
+ *   A = largest finite |x| of the block; e = the least integer with A * 2^-e <= 448, at least -126 (a block of zeros: -126);
+ *   code = e4m3(x * 2^-e), to nearest, ties to even (off by at most 2^-4 of the value, or 2^(e-10) where that is more); value = code * 2^e, exactly.
+ * An infinite or NaN number is held as NaN; the others of its block keep their precision. (A float32 above 248 * 2^120 = 3.297e38 is held as 2^128, which
+ * counts as infinity; in products, numbers below 2^-126 may count as 0.) A slot that was never written holds zeros.
+ *
+ * `*_dev` calls queue their work on `stream` (a hipStream_t of the context's device; NULL: the device's null stream; comet_ctx_stream(ctx): lane 0)
+ * and return. They allocate nothing and wait for nothing, so they can be captured into a HIP graph; a graph replays the pointers and sizes of the
+ * captured call. Calls on one store from several streams are the caller's to order (reads and products may overlap each other). Device arrays of any
+ * stride (`ld`, in elements) and any alignment down to the element's are taken. The host-array forms run on lane 0 and return when done. */
+typedef struct comet_fp8_rows comet_fp8_rows;
+typedef enum { COMET_F32 = 0, COMET_F16 = 1, COMET_BF16 = 2 } comet_dtype;
+COMET_API int comet_fp8_create(comet_ctx* ctx, int64_t capacity, int32_t dim, comet_fp8_rows** out);   /* capacity * dim <= 2^40; capacity * (128 * blocks + scales + 4) bytes of HBM */
+COMET_API int comet_fp8_destroy(comet_fp8_rows* rows);       /* before its context; waits for work in flight on the store */
+COMET_API int64_t comet_fp8_capacity(const comet_fp8_rows* rows);
+COMET_API int comet_fp8_dim(const comet_fp8_rows* rows);
+/* Row i of vecs (n x dim of `dtype`) goes to slot slots_dev[i], or first_slot + i when slots_dev is NULL. A slot outside [0, capacity) skips its row
+ * (first_slot is checked on the host instead); of rows with the same slot the last one stays, whole. */
+COMET_API int comet_fp8_write_dev(comet_fp8_rows* rows, const int64_t* slots_dev, int64_t first_slot, const void* vecs_dev, int dtype, int64_t ld, int64_t n,
+                                  void* stream);
+/* out[i] (n x dim of `dtype`, rounded once from the exact value) = the row in slot slots_dev[i], or first_slot + i; zeros for a slot outside [0, capacity).
+ * Columns of out from dim to ld are left as they were. */
+COMET_API int comet_fp8_read_dev(const comet_fp8_rows* rows, const int64_t* slots_dev, int64_t first_slot, void* out_dev, int dtype, int64_t ld, int64_t n, void* stream);
+/* host arrays; a slot outside [0, capacity) is an error and nothing is written */
+COMET_API int comet_fp8_write(comet_fp8_rows* rows, const int64_t* slots, const float* vecs, int64_t n);
+COMET_API int comet_fp8_read(const comet_fp8_rows* rows, const int64_t* slots, int64_t n, float* out);
+/* Scores: out[i][j] (m x n of `dtype`) = inner product of slot q_first + i of `queries` with slot first + j of `rows`, products and scales exact, sums in
+ * float32, rounded once to `dtype`. Queries are quantised by writing them to a store of their own (a store may also be multiplied with itself). */
+COMET_API int comet_fp8_scores_dev(const comet_fp8_rows* queries, int64_t q_first, int64_t m, const comet_fp8_rows* rows, int64_t first, int64_t n, void* out_dev,
+                                   int dtype, int64_t ld, void* stream);
+
+/* Rows of scores as distributions, p_j = softmax(scale * s)_j: for each of m rows, over its first count columns (counts_dev[i] clamped to [0, n], or n
+ * when counts_dev is NULL; entries behind them are not read),
+ *   logsum = log sum_j exp(scale * s_j), entropy = -sum_j p_j log p_j (natural logarithms), logprobs (m x n_targets) = log p of the columns targets_dev[i][*],
+ *   ids / top_logprobs (m x k) = the k columns of largest scale * s_j and their log p; equal scores: the lower column first. k <= 128.
+ * scale may be negative (distances: the smallest are the best), not 0. An entry whose scaled score is -inf is masked: probability 0, never among the ids.
+ * Places no column is left for hold id -1 and log p -inf. A row with no unmasked entry: logsum -inf, entropy 0, log p -inf. A target outside [0, count):
+ * -inf. A row with a NaN or a scaled score of +inf among its entries: logsum, entropy and log p NaN; a NaN is never among the ids.
+ * n <= 2^30. `work_dev`: comet_logprobs_work_bytes(m, n, k) bytes (0 for short rows), 16-byte aligned, written and read by the call; the size for
+ * (m, n, k) is enough for every smaller m, n, k. Two calls that may run at once need two. */
+COMET_API int comet_logprobs_work_bytes(int64_t m, int64_t n, int32_t k, size_t* out_bytes);
+COMET_API int comet_logprobs_dev(comet_ctx* ctx, const void* scores_dev, int dtype, int64_t ld, int64_t m, int64_t n, const int32_t* counts_dev, float scale,
+                                 const int32_t* targets_dev, int32_t n_targets, int32_t k, float* out_logprobs_dev, float* out_logsum_dev, float* out_entropy_dev,
+                                 int32_t* out_ids_dev, float* out_top_logprobs_dev, void* work_dev, size_t work_bytes, void* stream);
+/* B queries (host, B x dim) against slots [first, first + n) of a store in one call: quantised as a write would, scored, and for each query the k slots of
+ * largest scale * score with their log-probabilities among the n (B x k), logsum and entropy (B). Host arrays. */
+COMET_API int comet_fp8_search(const comet_fp8_rows* rows, int64_t first, int64_t n, const float* queries, int32_t B, float scale, int32_t k, int64_t* out_slots,
+                               float* out_logprobs, float* out_logsum, float* out_entropy);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,65 @@
+"""What the 8-bit row store's entry points refuse before they touch a device, and the plain restatements the GPU tests compare with."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+import fp8_ref as ref
+from comet_amd import _lib
+
+
+def test_null_handles_are_refused():
+    lib = _lib.load()
+    h, z = C.c_void_p(), C.c_size_t()
+    assert lib.comet_fp8_create(None, 8, 8, C.byref(h)) == _lib.ERR_INVALID_ARG and not h.value and b"context" in lib.comet_last_error()
+    assert lib.comet_fp8_destroy(None) == _lib.OK
+    assert lib.comet_fp8_capacity(None) == 0 and lib.comet_fp8_dim(None) == 0
+    assert lib.comet_fp8_write_dev(None, None, 0, None, 0, 0, 0, None) == _lib.ERR_INVALID_ARG and b"rows must not be null" in lib.comet_last_error()
+    assert lib.comet_fp8_read_dev(None, None, 0, None, 0, 0, 0, None) == _lib.ERR_INVALID_ARG
+    assert lib.comet_fp8_scores_dev(None, 0, 0, None, 0, 0, None, 0, 0, None) == _lib.ERR_INVALID_ARG
+    assert lib.comet_fp8_write(None, None, None, 0) == _lib.ERR_INVALID_ARG
+    assert lib.comet_fp8_read(None, None, 0, None) == _lib.ERR_INVALID_ARG
+    assert lib.comet_fp8_search(None, 0, 0, None, 0, 1.0, 0, None, None, None, None) == _lib.ERR_INVALID_ARG
+    assert lib.comet_logprobs_dev(None, None, 0, 0, 0, 0, None, 1.0, None, 0, 0, None, None, None, None, None, None, 0, None) == _lib.ERR_INVALID_ARG
+    assert lib.comet_logprobs_work_bytes(1, 1, 1, None) == _lib.ERR_INVALID_ARG
+    for m, n, k in ((-1, 1, 1), (1, -1, 1), (1, (1 << 30) + 1, 1), (1, 1, -1), (1, 1, 129)):
+        assert lib.comet_logprobs_work_bytes(m, n, k, C.byref(z)) == _lib.ERR_INVALID_ARG, (m, n, k)
+
+
+def test_workspace_of_a_large_call_serves_smaller_ones():
+    lib = _lib.load()
+
+    def need(m, n, k):
+        z = C.c_size_t()
+        assert lib.comet_logprobs_work_bytes(m, n, k, C.byref(z)) == 0
+        return z.value
+    rng = np.random.default_rng(0)
+    for _ in range(500):
+        m, n, k = int(rng.integers(1, 5000)), int(rng.integers(1, 1 << 21)), int(rng.integers(0, 129))
+        a, b, c = int(rng.integers(1, m + 1)), int(rng.integers(1, n + 1)), int(rng.integers(0, k + 1))
+        assert need(a, b, c) <= need(m, n, k), ((a, b, c), (m, n, k))
+    assert need(1, 1000, 128) == 0 and need(0, 1 << 30, 128) == 0
+
+
+@pytest.mark.parametrize("seed", range(4))
+def test_reference_codes_are_the_nearest(seed):
+    """the plain quantiser against torch's own e4m3 conversion on scaled values, and its error bound"""
+    torch = pytest.importorskip("torch")
+    rng = np.random.default_rng(seed)
+    x = (rng.standard_normal((40, 300)) * np.exp(3 * rng.standard_normal((40, 300)))).astype(np.float32)
+    h = ref.held(x)
+    for c in range(0, 300, 128):
+        b, hb = x[:, c:c + 128].astype(np.float64), h[:, c:c + 128]
+        A = np.abs(b).max(axis=1)
+        e = np.array([min(i for i in range(-126, 121) if a * 2.0 ** -i <= 448) for a in A])
+        u = 2.0 ** e[:, None]
+        t = torch.from_numpy((b / u).astype(np.float32)).to(torch.float8_e4m3fn).to(torch.float64).numpy()
+        assert (hb == t * u).all()
+        assert (np.abs(hb - b) <= np.maximum(np.abs(b) * 2.0 ** -4, 2.0 ** -10 * u)).all()
+
+
+def test_reference_bf16_round_trip():
+    u = np.arange(0, 65536, dtype=np.uint32).astype(np.uint16)
+    f = ref.from_bf16_bits(u)
+    ok = ~np.isnan(f)
+    assert (ref.to_bf16_bits(f)[ok] == u[ok]).all()
