@@ -34,6 +34,19 @@ __device__ __forceinline__ v8b widen(int lo, int hi, float scale) {
     return v8b{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
+// four consecutive scores of one query; the only rounding behind the float32 sums
+template <class T> __device__ __forceinline__ void store4(T* row, int64_t j, int64_t n, v4f v) {
+    T o[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) o[i] = (T)v[i];
+    if (j + 4 <= n) {
+        __builtin_memcpy(row + j, o, sizeof(o));
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++) if (j + i < n) row[j + i] = o[i];
+    }
+}
+
 // Few queries: the stored rows stream once through the registers, each wave 64 rows (4 tiles of 16) against MT tiles of 16 queries, whose blocks come
 // out of the caches. Accumulator element i of lane l: row 4 * (l / 16) + i of its tile, query l % 16.
 template <class T, int MT>
@@ -97,19 +110,120 @@ __global__ __launch_bounds__(256) void scores_stream_kernel(const uint8_t* __res
         const int q = m0 + v * 16 + (lane & 15);
         if (q >= m) continue;
 #pragma unroll
-        for (int t = 0; t < RT; t++) {
-            const int64_t j = n0 + t * 16 + (lane >> 4) * 4;
-            T* dst = out + q * ld + j;
-            T o[4];
+        for (int t = 0; t < RT; t++) store4(out + q * ld, n0 + t * 16 + (lane >> 4) * 4, n, acc[t][v]);
+    }
+}
+
+// Many queries: a workgroup takes 128 queries x 128 rows, its four waves 64 x 64 each, and walks the blocks with both operands' codes in two LDS buffers that
+// are filled by the memory pipe itself: while one block is multiplied the next arrives. A tile of codes is 128 rows of eight 16-byte pieces; piece c of row r
+// lies at place c ^ (r & 7), so that the sixteen rows of an operand read fall on all banks (the fill permutes its global addresses, not its LDS ones).
+constexpr int kTile = 128, kTileBytes = kTile * kFp8Block;
+
+// The fill is an asm statement: around the compiler's own form of it every LDS read that follows would wait for the fill just issued (it cannot tell the two
+// buffers apart). The waits are written out where the buffers change hands. It has no register outputs; M0 holds the LDS address of the wave's 1 KiB.
+__device__ __forceinline__ void fill_1k(const uint8_t* base /* uniform */, uint32_t offset, uint32_t lds /* uniform */) {
+    const uint64_t b = (uint64_t)base;
+    const uint64_t sb = ((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(b >> 32)) << 32) | (uint32_t)__builtin_amdgcn_readfirstlane((int)b);
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %0, %1" :: "v"(offset), "s"(sb), "s"(__builtin_amdgcn_readfirstlane((int)lds)) : "memory");
+}
+// A wave's eighth-of-eight rows of a tile: instruction i fills rows (4 i + wave) * 8 .. + 7. offset[i]: the lane's 16 bytes relative to the tile's first row
+// (rows past the matrix's last read the last one).
+__device__ __forceinline__ void tile_offsets(int64_t first, int64_t count, int64_t row_bytes, uint32_t (&offset)[4]) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
-            for (int i = 0; i < 4; i++) o[i] = (T)acc[t][v][i];         // the only rounding behind the float32 sums
-            if (j + 4 <= n) {
-                __builtin_memcpy(dst, o, sizeof(o));
-            } else {
+    for (int i = 0; i < 4; i++) {
+        int64_t r = (i * 4 + wave) * 8 + (lane >> 3);
+        r = first + r < count ? r : count - 1 - first;
+        offset[i] = (uint32_t)(r * row_bytes) + ((lane & 7) ^ (lane >> 3)) * 16;
+    }
+}
+__device__ __forceinline__ void fill_tile(const uint8_t* base, const uint32_t (&offset)[4], uint32_t lds) {
+    const int wave = threadIdx.x >> 6;
 #pragma unroll
-                for (int i = 0; i < 4; i++) if (j + i < n) dst[i] = o[i];
+    for (int i = 0; i < 4; i++) fill_1k(base, offset[i], lds + (i * 4 + wave) * 1024);
+}
+__device__ __forceinline__ uint32_t lds_address(const void* p) { return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)p; }
+// a lane's two pieces of tile row r0 + lane % 16
+__device__ __forceinline__ v8i read_tile(const uint8_t* lds, int r0) {
+    const int lane = threadIdx.x & 63, r = r0 + (lane & 15), g = lane >> 4;
+    const uint8_t* p = lds + r * kFp8Block;
+    const v4i a = *(const v4i*)(p + ((g ^ (r & 7)) * 16)), b = *(const v4i*)(p + (((4 + g) ^ (r & 7)) * 16));
+    return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+
+template <class T>
+__global__ __launch_bounds__(256, 2) void scores_tile_kernel(const uint8_t* __restrict__ qc, const uint8_t* __restrict__ qs, int m, const uint8_t* __restrict__ rc,
+                                                             const uint8_t* __restrict__ rs, int n, int nb, int nb4, T* __restrict__ out, int64_t ld, int m_tiles, int n_tiles) {
+    __shared__ __align__(16) uint8_t lds[2][2][kTileBytes];
+    // Workgroups go to the eight XCDs in turn; each XCD takes a contiguous run of the tiles, queries fastest, so that a row tile is read into one L2.
+    const int tiles = m_tiles * n_tiles, per = (tiles + 7) / 8;
+    const int tile = (int)(blockIdx.x & 7) * per + (int)(blockIdx.x >> 3);
+    if (tile >= tiles) return;
+    const int64_t m0 = (int64_t)(tile % m_tiles) * kTile, n0 = (int64_t)(tile / m_tiles) * kTile;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int wm = (wave & 1) * 64, wn = (wave >> 1) * 64;
+    const int64_t row_bytes = (int64_t)nb * kFp8Block;
+    const uint8_t *qsp[4], *rsp[4];
+#pragma unroll
+    for (int t = 0; t < 4; t++) {
+        int64_t q = m0 + wm + t * 16 + (lane & 15), r = n0 + wn + t * 16 + (lane & 15);
+        qsp[t] = qs + (q < m ? q : m - 1) * nb4; rsp[t] = rs + (r < n ? r : n - 1) * nb4;
+    }
+    v4f acc[4][4];
+#pragma unroll
+    for (int t = 0; t < 4; t++)
+#pragma unroll
+        for (int v = 0; v < 4; v++) acc[t][v] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+    uint32_t qo[4], ro[4];
+    tile_offsets(m0, m, row_bytes, qo); tile_offsets(n0, n, row_bytes, ro);
+    const uint8_t *qb0 = qc + m0 * row_bytes, *rb0 = rc + n0 * row_bytes;
+    const uint32_t l0 = lds_address(&lds[0][0][0]);
+    uint32_t sr[4], sq[4], sr_next[4], sq_next[4];
+#pragma unroll
+    for (int t = 0; t < 4; t++) { sr_next[t] = *(const uint32_t*)rsp[t]; sq_next[t] = *(const uint32_t*)qsp[t]; }
+    fill_tile(qb0, qo, l0); fill_tile(rb0, ro, l0 + kTileBytes);
+    for (int b = 0; b < nb; b++) {
+        // this block and its scales have arrived for every wave, and every wave is done with the buffer that the next one goes to
+        asm volatile("s_waitcnt vmcnt(0)" : "+v"(sr_next[0]), "+v"(sr_next[1]), "+v"(sr_next[2]), "+v"(sr_next[3]), "+v"(sq_next[0]), "+v"(sq_next[1]), "+v"(sq_next[2]), "+v"(sq_next[3]) :: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        if ((b & 3) == 0) {
+#pragma unroll
+            for (int t = 0; t < 4; t++) { sr[t] = sr_next[t]; sq[t] = sq_next[t]; }
+        }
+        if (b + 1 < nb) {
+            const uint32_t to = l0 + ((b + 1) & 1) * (2 * kTileBytes);
+            fill_tile(qb0 + (b + 1) * kFp8Block, qo, to); fill_tile(rb0 + (b + 1) * kFp8Block, ro, to + kTileBytes);
+            if (((b + 1) & 3) == 0) {
+#pragma unroll
+                for (int t = 0; t < 4; t++) { sr_next[t] = *(const uint32_t*)(rsp[t] + b + 1); sq_next[t] = *(const uint32_t*)(qsp[t] + b + 1); }
             }
         }
+        const uint8_t *lq = lds[b & 1][0], *lr = lds[b & 1][1];
+        v8i r[4], q[4];
+        float fr[4], fq[4];
+#pragma unroll
+        for (int t = 0; t < 4; t++) {
+            r[t] = read_tile(lr, wn + t * 16); q[t] = read_tile(lq, wm + t * 16);
+            fr[t] = scale_of(sr[t], b & 3); fq[t] = scale_of(sq[t], b & 3);
+        }
+#pragma unroll
+        for (int w = 0; w < 4; w++) {
+            v8b qb[4], rb[4];
+#pragma unroll
+            for (int t = 0; t < 4; t++) { qb[t] = widen(q[t][2 * w], q[t][2 * w + 1], fq[t]); rb[t] = widen(r[t][2 * w], r[t][2 * w + 1], fr[t]); }
+#pragma unroll
+            for (int t = 0; t < 4; t++)
+#pragma unroll
+                for (int v = 0; v < 4; v++) acc[t][v] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(rb[t], qb[v], acc[t][v], 0, 0, 0);
+        }
+    }
+#pragma unroll
+    for (int v = 0; v < 4; v++) {
+        const int64_t q = m0 + wm + v * 16 + (lane & 15);
+        if (q >= m) continue;
+#pragma unroll
+        for (int t = 0; t < 4; t++) store4(out + q * ld, n0 + wn + t * 16 + (lane >> 4) * 4, n, acc[t][v]);
     }
 }
 
@@ -123,8 +237,8 @@ template <class T> void scores_t(hipStream_t s, const Fp8View& q, int64_t q_firs
         const int64_t nt = ceil_div(nj, 256);
         if (mi <= 16) hipLaunchKernelGGL((scores_stream_kernel<T, 1>), dim3((unsigned)nt), dim3(256), 0, s, qc, qs, mi, rc, rs, nj, r.nb, r.nb4, o, ld, 1);
         else {
-            const int mt = (int)ceil_div(mi, 64);
-            hipLaunchKernelGGL((scores_stream_kernel<T, 4>), dim3((unsigned)(nt * mt)), dim3(256), 0, s, qc, qs, mi, rc, rs, nj, r.nb, r.nb4, o, ld, mt);
+            const int mt = (int)ceil_div(mi, kTile), ntile = (int)ceil_div(nj, kTile);
+            hipLaunchKernelGGL((scores_tile_kernel<T>), dim3((unsigned)(ceil_div((int64_t)mt * ntile, 8) * 8)), dim3(256), 0, s, qc, qs, mi, rc, rs, nj, r.nb, r.nb4, o, ld, mt, ntile);
         }
         LAUNCH_CHECK();
     }
