@@ -13,13 +13,13 @@
 namespace comet {
 namespace {
 
-constexpr int kThreads = 256, kEpt = 32, kChunk = kThreads * kEpt;
-// candidate buffer: the k best so far and one chunk's survivors. When more than kSoft would be held, the chunk is cut to the keys not below the k-th
+constexpr int kThreads = 256, kWaves = kThreads / 64, kEpt = 16, kChunk = kThreads * kEpt;
+// Candidate buffer: the k best so far and one chunk's survivors. When more than kSoft would be held, the chunk is cut to the keys not below the k-th
 // largest of the 256 threads' largest keys: only the k threads above that bound hold survivors, kEpt each.
-constexpr int kSoft = 1024, kCap = kLogProbsMaxK + kEpt * kLogProbsMaxK;
+constexpr int kSoft = 512, kCap = kLogProbsMaxK + kEpt * kLogProbsMaxK;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
-struct Stats { float m, s, w; int bad; };   // maximum, S, W in units of log2 (w = sum e * t, t = d * log2 e); bad: a NaN was seen
+struct Stats { float m, s, w; int bad; };   // maximum, S, W in units of log2 (w = sum e * t, t = d * log2 e); bad: a NaN among masked entries only (any other is in s)
 
 __device__ __forceinline__ float exp2_t(float t) { return __builtin_amdgcn_exp2f(t); }
 
@@ -27,10 +27,8 @@ __device__ __forceinline__ void stats_join(Stats& a, float m, float s, float w, 
     a.bad |= bad;
     const float hi = fmaxf(a.m, m);
     if (hi == -INFINITY) return;
-    float ta = (a.m - hi) * f, tb = (m - hi) * f;
-    ta = ta < -1e30f ? -1e30f : ta; tb = tb < -1e30f ? -1e30f : tb;      // -inf * 0 below would be NaN
-    const float ea = exp2_t(ta), eb = exp2_t(tb);
-    a.w = (a.w + ta * a.s) * ea + (w + tb * s) * eb;
+    const float ta = (a.m - hi) * f, tb = (m - hi) * f, ea = exp2_t(ta), eb = exp2_t(tb);
+    a.w = (a.w + fmaxf(ta, -1e30f) * a.s) * ea + (w + fmaxf(tb, -1e30f) * s) * eb;       // -inf * 0 would be NaN; a NaN stays in ea, eb
     a.s = a.s * ea + s * eb;
     a.m = hi;
 }
@@ -45,57 +43,87 @@ __device__ __forceinline__ uint64_t make_key(float x, uint32_t col) { return ((u
 __device__ __forceinline__ uint32_t key_col(uint64_t k) { return 0xFFFFFFFFu - (uint32_t)k; }
 
 struct Shared {
-    uint64_t buf[kCap];
-    uint64_t best[kThreads];
+    alignas(16) uint64_t buf[kCap];
+    alignas(16) uint64_t best[kThreads];
     uint64_t cut;
-    int total[kThreads / 64];
-    int cnt;
-    float sm[kThreads / 64], ss[kThreads / 64], sw[kThreads / 64]; int sb[kThreads / 64];
+    int total[2][kWaves];
+    float sm[kWaves], ss[kWaves], sw[kWaves]; int sb[kWaves];
     Stats row;
 };
 
-// buf[0 .. cnt) sorted descending, cut to k; every thread returns the new count
-__device__ int compact(Shared& sh, int cnt, int k) {
-    int p = 64;
-    while (p < cnt) p <<= 1;                 // at most 8192 > kCap: the pad beyond kCap is never stored (see below)
-    const int top = p < kCap ? p : kCap;
-    for (int i = cnt + threadIdx.x; i < top; i += kThreads) sh.buf[i] = 0;
+struct TopK { int cnt = 0; uint64_t thr = 0; bool sorted = true; int turn = 0; };    // the same in every thread; thr: the k-th best key so far (0: none)
+
+// buf[0 .. cnt) sorted descending and cut to k. Up to 512 keys each thread counts the keys above its own two (two LDS reads of a pair per step, all lanes
+// the same address); more, which takes rows whose best columns crowd into few threads, go through a bitonic network.
+__device__ void compact(Shared& sh, TopK& tk, int k) {
+    const int cnt = tk.cnt;
     __syncthreads();
-    for (int size = 2; size <= p; size <<= 1) {
-        for (int stride = size >> 1; stride > 0; stride >>= 1) {
-            for (int t = threadIdx.x; t < p / 2; t += kThreads) {
-                const int i = 2 * t - (t & (stride - 1)), j = i + stride;
-                // bitonic network with every merge descending: the first step of a merge compares mirrored positions
-                const int jj = stride == (size >> 1) ? (i & ~(size - 1)) + size - 1 - (i & (size - 1)) : j;
-                const int lo = i < jj ? i : jj, hi = i < jj ? jj : i;
-                if (hi < kCap) {             // positions from kCap on hold 0, the smallest key: nothing moves there
-                    const uint64_t a = sh.buf[lo], b = sh.buf[hi];
-                    if (a < b) { sh.buf[lo] = b; sh.buf[hi] = a; }
+    if (cnt <= 2 * kThreads) {
+        const int a = threadIdx.x, b = a + kThreads;
+        const uint64_t ka = a < cnt ? sh.buf[a] : 0, kb = b < cnt ? sh.buf[b] : 0;
+        int ra = 0, rb = 0;
+        const ulonglong2* pair = (const ulonglong2*)sh.buf;
+        if (cnt <= kThreads) {
+#pragma unroll 4
+            for (int j = 0; j < cnt / 2; j++) { const ulonglong2 q = pair[j]; ra += (q.x > ka) + (q.y > ka); }
+            if (cnt & 1) ra += sh.buf[cnt - 1] > ka;
+        } else {
+#pragma unroll 4
+            for (int j = 0; j < cnt / 2; j++) { const ulonglong2 q = pair[j]; ra += (q.x > ka) + (q.y > ka); rb += (q.x > kb) + (q.y > kb); }
+            if (cnt & 1) { const uint64_t q = sh.buf[cnt - 1]; ra += q > ka; rb += q > kb; }
+        }
+        __syncthreads();
+        if (a < cnt && ra < k) sh.buf[ra] = ka;
+        if (b < cnt && rb < k) sh.buf[rb] = kb;
+        __syncthreads();
+    } else {
+        int p = 1024;
+        while (p < cnt) p <<= 1;                 // at most 8192; positions from kCap on are never stored and hold 0, the smallest key
+        for (int i = cnt + threadIdx.x; i < (p < kCap ? p : kCap); i += kThreads) sh.buf[i] = 0;
+        __syncthreads();
+        for (int size = 2; size <= p; size <<= 1) {
+            for (int stride = size >> 1; stride > 0; stride >>= 1) {
+                for (int t = threadIdx.x; t < p / 2; t += kThreads) {
+                    // every merge descending: its first step compares mirrored positions
+                    const int i = 2 * t - (t & (stride - 1));
+                    const int j = stride == (size >> 1) ? (i & ~(size - 1)) + size - 1 - (i & (size - 1)) : i + stride;
+                    if (j < kCap) { const uint64_t x = sh.buf[i], y = sh.buf[j]; if (x < y) { sh.buf[i] = y; sh.buf[j] = x; } }
                 }
+                __syncthreads();
             }
-            __syncthreads();
         }
     }
-    return cnt < k ? cnt : k;
+    tk.cnt = cnt < k ? cnt : k;
+    tk.sorted = true;
+    if (cnt >= k) tk.thr = sh.buf[k - 1];
 }
 
-// Adds this chunk's candidates: bit i of `mask` says that element i of this thread is one, key(i) is its key. thr_key: the k-th best key so far (0: none).
-// Uniform across the workgroup; returns the number held.
-template <int EPT, class Key>
-__device__ int add_candidates(Shared& sh, int cnt, int k, uint32_t mask, Key key, uint64_t& thr_key) {
+// the number of set bits in the lower threads' masks (before) and in all of them
+__device__ __forceinline__ int count_bits(Shared& sh, TopK& tk, uint32_t mask, int& before) {
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    int c = __popc(mask);
+    const int mine = __popc(mask);
+    int scan = mine;
+    if (__ballot(mask != 0)) {
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) c += __shfl_xor(c, o, 64);
-    if (lane == 0) sh.total[wave] = c;
+        for (int o = 1; o < 64; o <<= 1) { const int x = __shfl_up(scan, o, 64); scan += lane >= o ? x : 0; }
+    }
+    int* total = sh.total[tk.turn ^= 1];          // two in turn: the other's readers have passed this barrier before it is written again
+    if (lane == 63) total[wave] = scan;
     __syncthreads();
-    c = 0;
+    int all = 0;
+    before = scan - mine;
 #pragma unroll
-    for (int w = 0; w < kThreads / 64; w++) c += sh.total[w];
-    if (c == 0) { __syncthreads(); return cnt; }
-    uint64_t cut = 0;
-    if (cnt + c > kSoft) {
-        if (cnt > k) { cnt = compact(sh, cnt, k); thr_key = cnt == k ? sh.buf[k - 1] : thr_key; }
+    for (int w = 0; w < kWaves; w++) { const int x = total[w]; all += x; before += w < wave ? x : 0; }
+    return all;
+}
+
+// Adds this chunk's candidates: bit i of `mask` says that element i of this thread is one, key(i) is its key.
+template <int EPT, class Key>
+__device__ void add_candidates(Shared& sh, TopK& tk, int k, uint32_t mask, Key key) {
+    int before, c = count_bits(sh, tk, mask, before);
+    if (c == 0) return;
+    if (tk.cnt + c > kSoft) {
+        if (tk.cnt > k) compact(sh, tk, k);
         uint64_t mine = 0;
 #pragma unroll
         for (int i = 0; i < EPT; i++) if ((mask >> i) & 1u) { const uint64_t q = key(i); mine = q > mine ? q : mine; }
@@ -103,27 +131,23 @@ __device__ int add_candidates(Shared& sh, int cnt, int k, uint32_t mask, Key key
         if (threadIdx.x == 0) sh.cut = 0;
         __syncthreads();
         int above = 0;
-        for (int t = 0; t < kThreads; t++) above += sh.best[t] > mine ? 1 : 0;
+        const ulonglong2* pair = (const ulonglong2*)sh.best;
+#pragma unroll 8
+        for (int t = 0; t < kThreads / 2; t++) { const ulonglong2 q = pair[t]; above += (q.x > mine) + (q.y > mine); }
         if (mine != 0 && above == k - 1) sh.cut = mine;       // keys are unique: at most one thread; nobody when fewer than k threads hold any
         __syncthreads();
-        cut = sh.cut;
-        cut = cut > thr_key ? cut : thr_key;
-    }
-    if (threadIdx.x == 0) sh.cnt = cnt;
-    __syncthreads();
+        uint64_t cut = sh.cut;
+        cut = cut > tk.thr ? cut : tk.thr;
 #pragma unroll
-    for (int i = 0; i < EPT; i++) if ((mask >> i) & 1u) {
-        const uint64_t q = key(i);
-        if (q >= cut) sh.buf[atomicAdd(&sh.cnt, 1)] = q;
+        for (int i = 0; i < EPT; i++) if (((mask >> i) & 1u) && key(i) < cut) mask &= ~(1u << i);
+        c = count_bits(sh, tk, mask, before);
     }
-    __syncthreads();
-    cnt = sh.cnt;
-    if ((thr_key == 0 && cnt >= k) || cnt >= k + kThreads) {
-        cnt = compact(sh, cnt, k);
-        if (cnt == k) thr_key = sh.buf[k - 1];
-    }
-    __syncthreads();
-    return cnt;
+    uint64_t* to = sh.buf + tk.cnt + before;
+#pragma unroll
+    for (int i = 0; i < EPT; i++) if ((mask >> i) & 1u) *to++ = key(i);
+    tk.cnt += c;
+    tk.sorted = false;
+    if ((tk.thr == 0 && tk.cnt >= k) || tk.cnt >= k + kThreads) compact(sh, tk, k);
 }
 
 __device__ void reduce_stats(Shared& sh, Stats st, float f) {
@@ -140,13 +164,11 @@ __device__ void reduce_stats(Shared& sh, Stats st, float f) {
     __syncthreads();
 }
 
-template <class T> __device__ __forceinline__ float flip_score(T v, uint32_t sign) {     // -0 becomes +0: the two are one score
-    return __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, (float)v) ^ sign) + 0.0f;
-}
+template <class T> __device__ __forceinline__ float signed_score(T v, float sign) { return __builtin_fmaf((float)v, sign, 0.0f); }     // sign: +-1; -0 becomes +0: the two are one score
 
 // a row's outputs from its statistics and its sorted best keys (sh.row, sh.buf[0 .. cnt))
 template <class T>
-__device__ void finish_row(Shared& sh, int64_t row, const T* x, int count, int cnt, const int32_t* targets, int n_targets, int k, float scale, uint32_t sign,
+__device__ void finish_row(Shared& sh, int64_t row, const T* x, int count, int cnt, const int32_t* targets, int n_targets, int k, float scale, float sign,
                            float* logprobs, float* logsum, float* entropy, int32_t* ids, float* top_logprobs) {
     const Stats st = sh.row;
     const bool empty = !st.bad && st.m == -INFINITY;
@@ -159,7 +181,7 @@ __device__ void finish_row(Shared& sh, int64_t row, const T* x, int count, int c
     for (int t = threadIdx.x; t < n_targets; t += kThreads) {
         const int32_t col = targets[row * n_targets + t];
         float v = -INFINITY;
-        if (!empty && col >= 0 && col < count) v = (flip_score(x[col], sign) - st.m) * scale - log_s;
+        if (!empty && col >= 0 && col < count) v = (signed_score(x[col], sign) - st.m) * scale - log_s;
         logprobs[row * n_targets + t] = v;
     }
     for (int i = threadIdx.x; i < k; i += kThreads) {
@@ -172,7 +194,7 @@ __device__ void finish_row(Shared& sh, int64_t row, const T* x, int count, int c
 
 // Workgroup (row, split): columns [split * span, ...) of the row's count in chunks of 8192, each thread 32 of them in 16-byte pieces.
 template <class T>
-__global__ __launch_bounds__(kThreads) void logprobs_kernel(const T* __restrict__ scores, int64_t ld, int n, const int32_t* __restrict__ counts, float scale, uint32_t sign,
+__global__ __launch_bounds__(kThreads) void logprobs_kernel(const T* __restrict__ scores, int64_t ld, int n, const int32_t* __restrict__ counts, float scale, float sign,
                                                             const int32_t* __restrict__ targets, int n_targets, int k, int splits, float* __restrict__ logprobs,
                                                             float* __restrict__ logsum, float* __restrict__ entropy, int32_t* __restrict__ ids, float* __restrict__ top_logprobs,
                                                             Stats* __restrict__ part_stats, uint64_t* __restrict__ part_keys) {
@@ -187,63 +209,67 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(const T* __restrict_
     const T* x = scores + row * ld;
     const float f = scale * kLog2e;
     Stats st{-INFINITY, 0.0f, 0.0f, 0};
-    int cnt = 0;
-    uint64_t thr_key = 0;
-    for (int c = split * per; c < c_end; c++) {
-        const int base = c * kChunk + threadIdx.x * V;
-        float v[kEpt];
-        if ((c + 1) * (int64_t)kChunk <= count) {
-            T t[P][V];
+    TopK tk;
+    const int whole = count / kChunk;
+    const T masked = (T)(-sign * INFINITY);
+    T next[P][V];          // the next chunk is requested before this one is worked on
+    auto fetch = [&](int c) {
+        const int64_t base = (int64_t)c * kChunk + threadIdx.x * V;
+        if (c < whole) {
 #pragma unroll
-            for (int p = 0; p < P; p++) __builtin_memcpy(t[p], x + base + p * (kThreads * V), 16);
+            for (int p = 0; p < P; p++) __builtin_memcpy(next[p], x + base + p * (kThreads * V), 16);
+        } else {
 #pragma unroll
             for (int p = 0; p < P; p++)
 #pragma unroll
-                for (int i = 0; i < V; i++) v[p * V + i] = flip_score(t[p][i], sign);
-        } else {
-#pragma unroll
-            for (int p = 0; p < P; p++) {
-                const int64_t col = (int64_t)base + p * (kThreads * V);
-                if (col + V <= count) {
-                    T t[V];
-                    __builtin_memcpy(t, x + col, 16);
-#pragma unroll
-                    for (int i = 0; i < V; i++) v[p * V + i] = flip_score(t[i], sign);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < V; i++) v[p * V + i] = col + i < count ? flip_score(x[col + i], sign) : -INFINITY;
-                }
-            }
+                for (int i = 0; i < V; i++) { const int64_t col = base + p * (kThreads * V) + i; next[p][i] = col < count ? x[col] : masked; }
         }
-        float hi = v[0];
+    };
+    int c = split * per;
+    if (c < c_end) fetch(c);
+    for (; c < c_end; c++) {
+        const int base = c * kChunk + threadIdx.x * V;
+        float v[kEpt];
 #pragma unroll
-        for (int i = 0; i < kEpt; i++) { st.bad |= v[i] != v[i] ? 1 : 0; hi = fmaxf(hi, v[i]); }
-        hi = fmaxf(hi, st.m);
-        if (hi > st.m && st.m > -INFINITY) {
-            float t = (st.m - hi) * f;
-            t = t < -1e30f ? -1e30f : t;
-            const float e = exp2_t(t);
-            st.w = (st.w + t * st.s) * e; st.s *= e;
-        }
-        st.m = hi;
+        for (int p = 0; p < P; p++)
+#pragma unroll
+            for (int i = 0; i < V; i++) v[p * V + i] = signed_score(next[p][i], sign);
+        if (c + 1 < c_end) fetch(c + 1);
+        float top = v[0];
+#pragma unroll
+        for (int i = 1; i < kEpt; i++) top = fmaxf(top, v[i]);       // leaves NaN out
+        const float hi = fmaxf(top, st.m);
         if (hi > -INFINITY) {
+            if (hi > st.m) {
+                if (st.m > -INFINITY) {
+                    const float t = (st.m - hi) * f, e = exp2_t(t);
+                    st.w = (st.w + fmaxf(t, -1e30f) * st.s) * e; st.s *= e;
+                }
+                st.m = hi;
+            }
+            float s = 0.0f, w = 0.0f;
 #pragma unroll
             for (int i = 0; i < kEpt; i++) {
-                float t = (v[i] - hi) * f;
-                t = t < -1e30f ? -1e30f : t;          // a masked entry, or one so far below that exp is 0 and t * 0 must be 0
-                const float e = exp2_t(t);
-                st.s += e; st.w = __builtin_fmaf(e, t, st.w);
+                const float t = (v[i] - hi) * f, e = exp2_t(t);
+                s += e; w = __builtin_fmaf(e, fmaxf(t, -1e30f), w);          // a masked entry: t = -inf, e = 0, and 0 * t must be 0; a NaN stays in e
             }
+            st.s += s; st.w += w;
+        } else {
+#pragma unroll
+            for (int i = 0; i < kEpt; i++) st.bad |= v[i] != v[i] ? 1 : 0;
         }
         if (k > 0) {
-            const float thr = thr_key ? unordered((uint32_t)(thr_key >> 32)) : -INFINITY;      // later columns lose a tie: strictly greater
+            const float thr = tk.thr ? unordered((uint32_t)(tk.thr >> 32)) : -INFINITY;      // later columns lose a tie: strictly greater
             uint32_t mask = 0;
+            if (__ballot(top > thr)) {
 #pragma unroll
-            for (int i = 0; i < kEpt; i++) mask |= v[i] > thr ? 1u << i : 0u;                  // false for NaN and for -inf
-            cnt = add_candidates<kEpt>(sh, cnt, k, mask, [&](int i) { return make_key(v[i], (uint32_t)(base + (i / V) * (kThreads * V) + i % V)); }, thr_key);
+                for (int i = 0; i < kEpt; i++) mask |= v[i] > thr ? 1u << i : 0u;              // false for NaN and for -inf
+            }
+            add_candidates<kEpt>(sh, tk, k, mask, [&](int i) { return make_key(v[i], (uint32_t)(base + (i / V) * (kThreads * V) + i % V)); });
         }
     }
-    if (k > 0) cnt = compact(sh, cnt, k);
+    if (k > 0 && !tk.sorted) compact(sh, tk, k);
+    const int cnt = tk.cnt;
     reduce_stats(sh, st, f);
     if (splits == 1) {
         finish_row(sh, row, x, count, cnt, targets, n_targets, k, scale, sign, logprobs, logsum, entropy, ids, top_logprobs);
@@ -255,7 +281,7 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(const T* __restrict_
 
 // joins a row's splits
 template <class T>
-__global__ __launch_bounds__(kThreads) void logprobs_join_kernel(const T* __restrict__ scores, int64_t ld, int n, const int32_t* __restrict__ counts, float scale, uint32_t sign,
+__global__ __launch_bounds__(kThreads) void logprobs_join_kernel(const T* __restrict__ scores, int64_t ld, int n, const int32_t* __restrict__ counts, float scale, float sign,
                                                                  const int32_t* __restrict__ targets, int n_targets, int k, int splits, float* __restrict__ logprobs,
                                                                  float* __restrict__ logsum, float* __restrict__ entropy, int32_t* __restrict__ ids, float* __restrict__ top_logprobs,
                                                                  const Stats* __restrict__ part_stats, const uint64_t* __restrict__ part_keys) {
@@ -267,18 +293,18 @@ __global__ __launch_bounds__(kThreads) void logprobs_join_kernel(const T* __rest
     const float f = scale * kLog2e;
     Stats st{-INFINITY, 0.0f, 0.0f, 0};
     for (int i = threadIdx.x; i < splits; i += kThreads) { const Stats p = part_stats[row * splits + i]; stats_join(st, p.m, p.s, p.w, p.bad, f); }
-    int cnt = 0;
-    uint64_t thr_key = 0;
+    TopK tk;
     const int total = splits * k;
     const uint64_t* keys = part_keys + row * total;
     for (int b = 0; b < total; b += kThreads * E) {
         uint64_t q[E];
         uint32_t mask = 0;
 #pragma unroll
-        for (int i = 0; i < E; i++) { const int at = b + i * kThreads + (int)threadIdx.x; q[i] = at < total ? keys[at] : 0; mask |= q[i] > thr_key ? 1u << i : 0u; }
-        cnt = add_candidates<E>(sh, cnt, k, mask, [&](int i) { return q[i]; }, thr_key);
+        for (int i = 0; i < E; i++) { const int at = b + i * kThreads + (int)threadIdx.x; q[i] = at < total ? keys[at] : 0; mask |= q[i] > tk.thr ? 1u << i : 0u; }
+        add_candidates<E>(sh, tk, k, mask, [&](int i) { return q[i]; });
     }
-    if (k > 0) cnt = compact(sh, cnt, k);
+    if (k > 0 && !tk.sorted) compact(sh, tk, k);
+    const int cnt = tk.cnt;
     reduce_stats(sh, st, f);
     finish_row(sh, row, scores + row * ld, count, cnt, targets, n_targets, k, scale, sign, logprobs, logsum, entropy, ids, top_logprobs);
 }
@@ -291,7 +317,7 @@ int split_count(int64_t m, int64_t n) {
 }
 
 template <class T> void logprobs_t(hipStream_t s, const LogProbsArgs& a) {
-    const uint32_t sign = a.scale < 0 ? 0x80000000u : 0u;
+    const float sign = a.scale < 0 ? -1.0f : 1.0f;
     const float scale = std::fabs(a.scale);
     constexpr int64_t kPiece = (int64_t)1 << 24;
     for (int64_t i = 0; i < a.m; i += kPiece) {
