@@ -51,41 +51,80 @@ struct Shared {
     Stats row;
 };
 
-struct TopK { int cnt = 0; uint64_t thr = 0; bool sorted = true; int turn = 0; };    // the same in every thread; thr: the k-th best key so far (0: none)
+struct TopK { int cnt = 0; uint64_t thr = 0; bool sorted = true; int turn = 0; };    // the same in every thread; thr: at least k of the keys so far are not below it (0: unknown)
 
-// buf[0 .. cnt) sorted descending and cut to k. Up to 512 keys each thread counts the keys above its own two (two LDS reads of a pair per step, all lanes
-// the same address); more, which takes rows whose best columns crowd into few threads, go through a bitonic network.
-__device__ void compact(Shared& sh, TopK& tk, int k) {
-    const int cnt = tk.cnt;
-    __syncthreads();
-    if (cnt <= 2 * kThreads) {
-        const int a = threadIdx.x, b = a + kThreads;
-        const uint64_t ka = a < cnt ? sh.buf[a] : 0, kb = b < cnt ? sh.buf[b] : 0;
-        int ra = 0, rb = 0;
-        const ulonglong2* pair = (const ulonglong2*)sh.buf;
-        if (cnt <= kThreads) {
-#pragma unroll 4
-            for (int j = 0; j < cnt / 2; j++) { const ulonglong2 q = pair[j]; ra += (q.x > ka) + (q.y > ka); }
-            if (cnt & 1) ra += sh.buf[cnt - 1] > ka;
-        } else {
-#pragma unroll 4
-            for (int j = 0; j < cnt / 2; j++) { const ulonglong2 q = pair[j]; ra += (q.x > ka) + (q.y > ka); rb += (q.x > kb) + (q.y > kb); }
-            if (cnt & 1) { const uint64_t q = sh.buf[cnt - 1]; ra += q > ka; rb += q > kb; }
+// the value of lane ^ X
+template <int X> __device__ __forceinline__ uint32_t xor_lane(uint32_t v) {
+    auto dpp = [](uint32_t x, auto ctrl) { return (uint32_t)__builtin_amdgcn_mov_dpp((int)x, decltype(ctrl)::value, 0xF, 0xF, true); };
+    if constexpr (X == 1) return dpp(v, std::integral_constant<int, 0xB1>{});                                                            // quads: 1 0 3 2
+    else if constexpr (X == 2) return dpp(v, std::integral_constant<int, 0x4E>{});                                                       // quads: 2 3 0 1
+    else if constexpr (X == 4) return dpp(dpp(v, std::integral_constant<int, 0x141>{}), std::integral_constant<int, 0x1B>{});            // eights mirrored, then quads
+    else if constexpr (X == 8) return dpp(v, std::integral_constant<int, 0x128>{});                                                      // sixteens turned by eight
+    else {
+        const auto r = X == 16 ? __builtin_amdgcn_permlane16_swap(v, v, false, false) : __builtin_amdgcn_permlane32_swap(v, v, false, false);
+        return (threadIdx.x & X) ? r[0] : r[1];
+    }
+}
+template <int X> __device__ __forceinline__ uint64_t xor_lane64(uint64_t v) { return ((uint64_t)xor_lane<X>((uint32_t)(v >> 32)) << 32) | xor_lane<X>((uint32_t)v); }
+
+// Sorts N * 256 keys descending, key i * 256 + thread in key[i] of that thread: a bitonic network whose strides below 64 are lane exchanges and whose strides
+// of 64 and 128 go through sh.best (256 keys are 33 lane steps and 3 of LDS; counting each key's rank instead was 64-bit compares of all with all, 8 us a
+// time with four workgroups on a CU).
+template <int N> __device__ void sort_keys(Shared& sh, uint64_t (&key)[N]) {
+    const int t = threadIdx.x;
+    auto keep = [&](uint64_t& mine, uint64_t other, bool lower, bool down) { mine = ((mine > other) == (lower == down)) ? mine : other; };
+    auto lanes = [&](auto X, int size) {
+        constexpr int x = decltype(X)::value;
+#pragma unroll
+        for (int i = 0; i < N; i++) keep(key[i], xor_lane64<x>(key[i]), (t & x) == 0, ((i * kThreads + t) & size) == 0);
+    };
+#pragma unroll
+    for (int size = 2; size <= N * kThreads; size <<= 1) {
+        if constexpr (N == 2) { if (size == 2 * kThreads) { const uint64_t a = key[0], b = key[1]; key[0] = a > b ? a : b; key[1] = a > b ? b : a; } }
+#pragma unroll
+        for (int stride = 128; stride >= 64; stride >>= 1) {
+            if (stride > size / 2) continue;
+#pragma unroll
+            for (int i = 0; i < N; i++) {
+                __syncthreads();
+                sh.best[t] = key[i];
+                __syncthreads();
+                keep(key[i], sh.best[t ^ stride], (t & stride) == 0, ((i * kThreads + t) & size) == 0);
+            }
         }
+        if (size >= 64) lanes(std::integral_constant<int, 32>{}, size);
+        if (size >= 32) lanes(std::integral_constant<int, 16>{}, size);
+        if (size >= 16) lanes(std::integral_constant<int, 8>{}, size);
+        if (size >= 8) lanes(std::integral_constant<int, 4>{}, size);
+        if (size >= 4) lanes(std::integral_constant<int, 2>{}, size);
+        lanes(std::integral_constant<int, 1>{}, size);
+    }
+}
+
+// buf[0 .. cnt) sorted descending and cut to k
+__device__ void compact(Shared& sh, TopK& tk, int k) {
+    const int cnt = tk.cnt, t = threadIdx.x;
+    __syncthreads();
+    if (cnt <= kThreads) {
+        uint64_t key[1] = {t < cnt ? sh.buf[t] : 0};
+        sort_keys<1>(sh, key);
+        if (t < k && t < cnt) sh.buf[t] = key[0];           // every thread has read its key before the sort's first barrier
         __syncthreads();
-        if (a < cnt && ra < k) sh.buf[ra] = ka;
-        if (b < cnt && rb < k) sh.buf[rb] = kb;
+    } else if (cnt <= 2 * kThreads) {
+        uint64_t key[2] = {sh.buf[t], t + kThreads < cnt ? sh.buf[t + kThreads] : 0};
+        sort_keys<2>(sh, key);
+        if (t < k) sh.buf[t] = key[0];                      // k <= 128 < 256 < cnt
         __syncthreads();
-    } else {
+    } else {                                                // rows whose best columns crowd into few threads
         int p = 1024;
-        while (p < cnt) p <<= 1;                 // at most 8192; positions from kCap on are never stored and hold 0, the smallest key
-        for (int i = cnt + threadIdx.x; i < (p < kCap ? p : kCap); i += kThreads) sh.buf[i] = 0;
+        while (p < cnt) p <<= 1;                            // positions from kCap on are never stored and hold 0, the smallest key
+        for (int i = cnt + t; i < (p < kCap ? p : kCap); i += kThreads) sh.buf[i] = 0;
         __syncthreads();
         for (int size = 2; size <= p; size <<= 1) {
             for (int stride = size >> 1; stride > 0; stride >>= 1) {
-                for (int t = threadIdx.x; t < p / 2; t += kThreads) {
+                for (int h = t; h < p / 2; h += kThreads) {
                     // every merge descending: its first step compares mirrored positions
-                    const int i = 2 * t - (t & (stride - 1));
+                    const int i = 2 * h - (h & (stride - 1));
                     const int j = stride == (size >> 1) ? (i & ~(size - 1)) + size - 1 - (i & (size - 1)) : i + stride;
                     if (j < kCap) { const uint64_t x = sh.buf[i], y = sh.buf[j]; if (x < y) { sh.buf[i] = y; sh.buf[j] = x; } }
                 }
@@ -98,56 +137,53 @@ __device__ void compact(Shared& sh, TopK& tk, int k) {
     if (cnt >= k) tk.thr = sh.buf[k - 1];
 }
 
-// the number of set bits in the lower threads' masks (before) and in all of them
-__device__ __forceinline__ int count_bits(Shared& sh, TopK& tk, uint32_t mask, int& before) {
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const int mine = __popc(mask);
-    int scan = mine;
-    if (__ballot(mask != 0)) {
+// Where the wave's candidates go: `take[i]` holds the lanes whose element i is one. Returns the workgroup's number of candidates, `before` those of the lower waves.
+template <int EPT> __device__ __forceinline__ int count_candidates(Shared& sh, TopK& tk, const uint64_t (&take)[EPT], int& before) {
+    const int wave = threadIdx.x >> 6;
+    int mine = 0;
 #pragma unroll
-        for (int o = 1; o < 64; o <<= 1) { const int x = __shfl_up(scan, o, 64); scan += lane >= o ? x : 0; }
-    }
+    for (int i = 0; i < EPT; i++) mine += __popcll(take[i]);
     int* total = sh.total[tk.turn ^= 1];          // two in turn: the other's readers have passed this barrier before it is written again
-    if (lane == 63) total[wave] = scan;
+    if ((threadIdx.x & 63) == 0) total[wave] = mine;
     __syncthreads();
     int all = 0;
-    before = scan - mine;
+    before = 0;
 #pragma unroll
     for (int w = 0; w < kWaves; w++) { const int x = total[w]; all += x; before += w < wave ? x : 0; }
     return all;
 }
 
-// Adds this chunk's candidates: bit i of `mask` says that element i of this thread is one, key(i) is its key.
+// Adds this chunk's candidates: take[i] holds the lanes whose element i is one (uniform across the wave), key(i) is its key.
 template <int EPT, class Key>
-__device__ void add_candidates(Shared& sh, TopK& tk, int k, uint32_t mask, Key key) {
-    int before, c = count_bits(sh, tk, mask, before);
+__device__ void add_candidates(Shared& sh, TopK& tk, int k, uint64_t (&take)[EPT], Key key) {
+    const int lane = threadIdx.x & 63;
+    int before, c = count_candidates(sh, tk, take, before);
     if (c == 0) return;
     if (tk.cnt + c > kSoft) {
         if (tk.cnt > k) compact(sh, tk, k);
-        uint64_t mine = 0;
+        uint64_t best[1] = {0};
 #pragma unroll
-        for (int i = 0; i < EPT; i++) if ((mask >> i) & 1u) { const uint64_t q = key(i); mine = q > mine ? q : mine; }
-        sh.best[threadIdx.x] = mine;
-        if (threadIdx.x == 0) sh.cut = 0;
+        for (int i = 0; i < EPT; i++) if ((take[i] >> lane) & 1) { const uint64_t q = key(i); best[0] = q > best[0] ? q : best[0]; }
+        sort_keys<1>(sh, best);
         __syncthreads();
-        int above = 0;
-        const ulonglong2* pair = (const ulonglong2*)sh.best;
-#pragma unroll 8
-        for (int t = 0; t < kThreads / 2; t++) { const ulonglong2 q = pair[t]; above += (q.x > mine) + (q.y > mine); }
-        if (mine != 0 && above == k - 1) sh.cut = mine;       // keys are unique: at most one thread; nobody when fewer than k threads hold any
+        if ((int)threadIdx.x == k - 1) sh.cut = best[0];      // the k-th largest, or 0 when fewer than k threads hold any
         __syncthreads();
-        uint64_t cut = sh.cut;
-        cut = cut > tk.thr ? cut : tk.thr;
+        // at least k keys are not below it: the bound for what follows, too
+        tk.thr = sh.cut > tk.thr ? sh.cut : tk.thr;
 #pragma unroll
-        for (int i = 0; i < EPT; i++) if (((mask >> i) & 1u) && key(i) < cut) mask &= ~(1u << i);
-        c = count_bits(sh, tk, mask, before);
+        for (int i = 0; i < EPT; i++) take[i] &= __ballot(key(i) >= tk.thr);
+        c = count_candidates(sh, tk, take, before);
     }
-    uint64_t* to = sh.buf + tk.cnt + before;
+    int at = tk.cnt + before;
 #pragma unroll
-    for (int i = 0; i < EPT; i++) if ((mask >> i) & 1u) *to++ = key(i);
+    for (int i = 0; i < EPT; i++) {
+        if (!take[i]) continue;
+        if ((take[i] >> lane) & 1) sh.buf[at + __builtin_amdgcn_mbcnt_hi((uint32_t)(take[i] >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)take[i], 0))] = key(i);
+        at += __popcll(take[i]);
+    }
     tk.cnt += c;
     tk.sorted = false;
-    if ((tk.thr == 0 && tk.cnt >= k) || tk.cnt >= k + kThreads) compact(sh, tk, k);
+    if (tk.cnt >= k + kThreads) compact(sh, tk, k);
 }
 
 __device__ void reduce_stats(Shared& sh, Stats st, float f) {
@@ -260,12 +296,11 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(const T* __restrict_
         }
         if (k > 0) {
             const float thr = tk.thr ? unordered((uint32_t)(tk.thr >> 32)) : -INFINITY;      // later columns lose a tie: strictly greater
-            uint32_t mask = 0;
-            if (__ballot(top > thr)) {
+            uint64_t take[kEpt];
+            const bool any = __ballot(top > thr) != 0;
 #pragma unroll
-                for (int i = 0; i < kEpt; i++) mask |= v[i] > thr ? 1u << i : 0u;              // false for NaN and for -inf
-            }
-            add_candidates<kEpt>(sh, tk, k, mask, [&](int i) { return make_key(v[i], (uint32_t)(base + (i / V) * (kThreads * V) + i % V)); });
+            for (int i = 0; i < kEpt; i++) take[i] = any ? __ballot(v[i] > thr) : 0;           // false for NaN and for -inf
+            add_candidates(sh, tk, k, take, [&](int i) { return make_key(v[i], (uint32_t)(base + (i / V) * (kThreads * V) + i % V)); });
         }
     }
     if (k > 0 && !tk.sorted) compact(sh, tk, k);
@@ -298,10 +333,12 @@ __global__ __launch_bounds__(kThreads) void logprobs_join_kernel(const T* __rest
     const uint64_t* keys = part_keys + row * total;
     for (int b = 0; b < total; b += kThreads * E) {
         uint64_t q[E];
-        uint32_t mask = 0;
+        uint64_t take[E];
 #pragma unroll
-        for (int i = 0; i < E; i++) { const int at = b + i * kThreads + (int)threadIdx.x; q[i] = at < total ? keys[at] : 0; mask |= q[i] > tk.thr ? 1u << i : 0u; }
-        add_candidates<E>(sh, tk, k, mask, [&](int i) { return q[i]; });
+        for (int i = 0; i < E; i++) { const int at = b + i * kThreads + (int)threadIdx.x; q[i] = at < total ? keys[at] : 0; }
+#pragma unroll
+        for (int i = 0; i < E; i++) take[i] = __ballot(q[i] > tk.thr);
+        add_candidates(sh, tk, k, take, [&](int i) { return q[i]; });
     }
     if (k > 0 && !tk.sorted) compact(sh, tk, k);
     const int cnt = tk.cnt;
