@@ -7,7 +7,7 @@
 //
 // The best k columns ride on the same pass: a workgroup keeps the candidates that exceed its k-th best so far in LDS and sorts them when they get many.
 // A key is (score, column) in 64 bits, larger is better, equal scores to the lower column; keys are unique, so the result does not depend on the order in
-// which candidates arrive. Bound by reading the scores once.
+// which candidates arrive. Candidates wait as the score's own bits over the column's complement and become keys when they are sorted. Bound by reading the scores once.
 #include "fp8.hpp"
 
 namespace comet {
@@ -15,7 +15,7 @@ namespace {
 
 constexpr int kThreads = 256, kWaves = kThreads / 64, kEpt = 16, kChunk = kThreads * kEpt;
 // Candidate buffer: the k best so far and one chunk's survivors. When more than kSoft would be held, the chunk is cut to the keys not below the k-th
-// largest of the 256 threads' largest keys: only the k threads above that bound hold survivors, kEpt each.
+// largest of the 256 threads' largest keys: only the k threads above that bound hold survivors, kEpt each. (Up to k = 32 quads of threads do.)
 constexpr int kSoft = 512, kCap = kLogProbsMaxK + kEpt * kLogProbsMaxK;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
@@ -39,12 +39,15 @@ __device__ __forceinline__ uint32_t ordered(float x) {
     return b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
 }
 __device__ __forceinline__ float unordered(uint32_t o) { return __builtin_bit_cast(float, o ^ ((uint32_t)((int32_t)~o >> 31) | 0x80000000u)); }
-__device__ __forceinline__ uint64_t make_key(float x, uint32_t col) { return ((uint64_t)ordered(x) << 32) | (0xFFFFFFFFu - col); }   // 0 is no key: it would need a NaN
-__device__ __forceinline__ uint32_t key_col(uint64_t k) { return 0xFFFFFFFFu - (uint32_t)k; }
+__device__ __forceinline__ uint64_t make_key(float x, uint32_t col) { return ((uint64_t)ordered(x + 0.0f /* -0 and 0 are one score */) << 32) | ~col; }   // 0 is no key: it would need a NaN
+__device__ __forceinline__ float key_score(uint64_t k) { return unordered((uint32_t)(k >> 32)); }
+__device__ __forceinline__ uint32_t key_col(uint64_t k) { return ~(uint32_t)k; }
 
 struct Shared {
-    alignas(16) uint64_t buf[kCap];
+    alignas(16) float score[kCap]; uint32_t col[kCap];      // the candidates
     alignas(16) uint64_t best[kThreads];
+    __device__ __forceinline__ uint64_t key(int i) const { return make_key(score[i], col[i]); }
+    __device__ __forceinline__ void put(int i, uint64_t k) { score[i] = key_score(k); col[i] = key_col(k); }
     uint64_t cut;
     int total[2][kWaves];
     float sm[kWaves], ss[kWaves], sw[kWaves]; int sb[kWaves];
@@ -101,32 +104,56 @@ template <int N> __device__ void sort_keys(Shared& sh, uint64_t (&key)[N]) {
     }
 }
 
-// buf[0 .. cnt) sorted descending and cut to k
+// the same for 64 keys in one wave
+__device__ __forceinline__ uint64_t sort_wave(uint64_t key) {
+    const int t = threadIdx.x & 63;
+    auto step = [&](auto X, int size) {
+        constexpr int x = decltype(X)::value;
+        const uint64_t other = xor_lane64<x>(key);
+        key = ((key > other) == (((t & x) == 0) == ((t & size) == 0))) ? key : other;
+    };
+#pragma unroll
+    for (int size = 2; size <= 64; size <<= 1) {
+        if (size >= 64) step(std::integral_constant<int, 32>{}, size);
+        if (size >= 32) step(std::integral_constant<int, 16>{}, size);
+        if (size >= 16) step(std::integral_constant<int, 8>{}, size);
+        if (size >= 8) step(std::integral_constant<int, 4>{}, size);
+        if (size >= 4) step(std::integral_constant<int, 2>{}, size);
+        step(std::integral_constant<int, 1>{}, size);
+    }
+    return key;
+}
+
+// the candidates 0 .. cnt sorted descending and cut to k
 __device__ void compact(Shared& sh, TopK& tk, int k) {
     const int cnt = tk.cnt, t = threadIdx.x;
     __syncthreads();
-    if (cnt <= kThreads) {
-        uint64_t key[1] = {t < cnt ? sh.buf[t] : 0};
+    if (cnt <= 64) {
+        if (t < 64) {
+            const uint64_t key = sort_wave(t < cnt ? sh.key(t) : 0);
+            if (t < cnt) sh.put(t, key);
+        }
+        __syncthreads();
+    } else if (cnt <= kThreads) {
+        uint64_t key[1] = {t < cnt ? sh.key(t) : 0};
         sort_keys<1>(sh, key);
-        if (t < k && t < cnt) sh.buf[t] = key[0];           // every thread has read its key before the sort's first barrier
+        if (t < k && t < cnt) sh.put(t, key[0]);            // every thread has read its key before the sort's first barrier
         __syncthreads();
     } else if (cnt <= 2 * kThreads) {
-        uint64_t key[2] = {sh.buf[t], t + kThreads < cnt ? sh.buf[t + kThreads] : 0};
+        uint64_t key[2] = {sh.key(t), t + kThreads < cnt ? sh.key(t + kThreads) : 0};
         sort_keys<2>(sh, key);
-        if (t < k) sh.buf[t] = key[0];                      // k <= 128 < 256 < cnt
+        if (t < k) sh.put(t, key[0]);                       // k <= 128 < 256 < cnt
         __syncthreads();
     } else {                                                // rows whose best columns crowd into few threads
         int p = 1024;
-        while (p < cnt) p <<= 1;                            // positions from kCap on are never stored and hold 0, the smallest key
-        for (int i = cnt + t; i < (p < kCap ? p : kCap); i += kThreads) sh.buf[i] = 0;
-        __syncthreads();
+        while (p < cnt) p <<= 1;                            // positions from cnt on are never stored and hold the smallest key
         for (int size = 2; size <= p; size <<= 1) {
             for (int stride = size >> 1; stride > 0; stride >>= 1) {
                 for (int h = t; h < p / 2; h += kThreads) {
                     // every merge descending: its first step compares mirrored positions
                     const int i = 2 * h - (h & (stride - 1));
                     const int j = stride == (size >> 1) ? (i & ~(size - 1)) + size - 1 - (i & (size - 1)) : i + stride;
-                    if (j < kCap) { const uint64_t x = sh.buf[i], y = sh.buf[j]; if (x < y) { sh.buf[i] = y; sh.buf[j] = x; } }
+                    if (j < cnt) { const uint64_t x = sh.key(i), y = sh.key(j); if (x < y) { sh.put(i, y); sh.put(j, x); } }
                 }
                 __syncthreads();
             }
@@ -134,7 +161,7 @@ __device__ void compact(Shared& sh, TopK& tk, int k) {
     }
     tk.cnt = cnt < k ? cnt : k;
     tk.sorted = true;
-    if (cnt >= k) tk.thr = sh.buf[k - 1];
+    if (cnt >= k) tk.thr = sh.key(k - 1);
 }
 
 // Where the wave's candidates go: `take[i]` holds the lanes whose element i is one. Returns the workgroup's number of candidates, `before` those of the lower waves.
@@ -153,32 +180,43 @@ template <int EPT> __device__ __forceinline__ int count_candidates(Shared& sh, T
     return all;
 }
 
-// Adds this chunk's candidates: take[i] holds the lanes whose element i is one (uniform across the wave), key(i) is its key.
-template <int EPT, class Key>
-__device__ void add_candidates(Shared& sh, TopK& tk, int k, uint64_t (&take)[EPT], Key key) {
+// Adds this chunk's candidates: take[i] holds the lanes whose element i is one (uniform across the wave). Of `chunk`: best() is the thread's largest key (0:
+// none), keep(cut, take) drops what lies below cut, score(i) and col(i) are an element.
+template <int EPT, class Chunk>
+__device__ __forceinline__ void add_candidates(Shared& sh, TopK& tk, int k, uint64_t (&take)[EPT], const Chunk& chunk) {
     const int lane = threadIdx.x & 63;
     int before, c = count_candidates(sh, tk, take, before);
     if (c == 0) return;
     if (tk.cnt + c > kSoft) {
         if (tk.cnt > k) compact(sh, tk, k);
-        uint64_t best[1] = {0};
-#pragma unroll
-        for (int i = 0; i < EPT; i++) if ((take[i] >> lane) & 1) { const uint64_t q = key(i); best[0] = q > best[0] ? q : best[0]; }
-        sort_keys<1>(sh, best);
-        __syncthreads();
-        if ((int)threadIdx.x == k - 1) sh.cut = best[0];      // the k-th largest, or 0 when fewer than k threads hold any
-        __syncthreads();
+        uint64_t best[1] = {chunk.best()};
+        if (k <= kThreads / 8) {
+            // quads stand for their threads: the k quads above the bound hold 4 * EPT keys each, and 64 keys sort in one wave
+            const uint64_t p = xor_lane64<1>(best[0]), a = best[0] > p ? best[0] : p, q = xor_lane64<2>(a), quad = a > q ? a : q;
+            if ((threadIdx.x & 3) == 0) sh.best[threadIdx.x >> 2] = quad;
+            __syncthreads();
+            if (threadIdx.x < 64) {
+                const uint64_t key = sort_wave(sh.best[threadIdx.x]);
+                if ((int)threadIdx.x == k - 1) sh.cut = key;
+            }
+        } else {
+            sort_keys<1>(sh, best);
+            if ((int)threadIdx.x == k - 1) sh.cut = best[0];
+        }
+        __syncthreads();                                      // sh.cut: the k-th largest, or 0 when fewer than k threads (quads) hold any
         // at least k keys are not below it: the bound for what follows, too
         tk.thr = sh.cut > tk.thr ? sh.cut : tk.thr;
-#pragma unroll
-        for (int i = 0; i < EPT; i++) take[i] &= __ballot(key(i) >= tk.thr);
+        chunk.keep(tk.thr, take);
         c = count_candidates(sh, tk, take, before);
     }
     int at = tk.cnt + before;
 #pragma unroll
     for (int i = 0; i < EPT; i++) {
         if (!take[i]) continue;
-        if ((take[i] >> lane) & 1) sh.buf[at + __builtin_amdgcn_mbcnt_hi((uint32_t)(take[i] >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)take[i], 0))] = key(i);
+        if ((take[i] >> lane) & 1) {
+            const int to = (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(take[i] >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)take[i], (uint32_t)at));
+            sh.score[to] = chunk.score(i); sh.col[to] = chunk.col(i);
+        }
         at += __popcll(take[i]);
     }
     tk.cnt += c;
@@ -200,11 +238,11 @@ __device__ void reduce_stats(Shared& sh, Stats st, float f) {
     __syncthreads();
 }
 
-template <class T> __device__ __forceinline__ float signed_score(T v, float sign) { return __builtin_fmaf((float)v, sign, 0.0f); }     // sign: +-1; -0 becomes +0: the two are one score
+template <bool NEG, class T> __device__ __forceinline__ float signed_score(T v) { return NEG ? -(float)v : (float)v; }
 
-// a row's outputs from its statistics and its sorted best keys (sh.row, sh.buf[0 .. cnt))
-template <class T>
-__device__ void finish_row(Shared& sh, int64_t row, const T* x, int count, int cnt, const int32_t* targets, int n_targets, int k, float scale, float sign,
+// a row's outputs from its statistics and its sorted best keys (sh.row, the sorted candidates 0 .. cnt)
+template <bool NEG, class T>
+__device__ void finish_row(Shared& sh, int64_t row, const T* x, int count, int cnt, const int32_t* targets, int n_targets, int k, float scale,
                            float* logprobs, float* logsum, float* entropy, int32_t* ids, float* top_logprobs) {
     const Stats st = sh.row;
     const bool empty = !st.bad && st.m == -INFINITY;
@@ -217,20 +255,19 @@ __device__ void finish_row(Shared& sh, int64_t row, const T* x, int count, int c
     for (int t = threadIdx.x; t < n_targets; t += kThreads) {
         const int32_t col = targets[row * n_targets + t];
         float v = -INFINITY;
-        if (!empty && col >= 0 && col < count) v = (signed_score(x[col], sign) - st.m) * scale - log_s;
+        if (!empty && col >= 0 && col < count) v = (signed_score<NEG>(x[col]) - st.m) * scale - log_s;
         logprobs[row * n_targets + t] = v;
     }
     for (int i = threadIdx.x; i < k; i += kThreads) {
         const bool has = i < cnt;
-        const uint64_t q = has ? sh.buf[i] : 0;
-        ids[row * k + i] = has ? (int32_t)key_col(q) : -1;
-        top_logprobs[row * k + i] = has ? (unordered((uint32_t)(q >> 32)) - st.m) * scale - log_s : -INFINITY;
+        ids[row * k + i] = has ? (int32_t)sh.col[i] : -1;
+        top_logprobs[row * k + i] = has ? (sh.score[i] - st.m) * scale - log_s : -INFINITY;
     }
 }
 
 // Workgroup (row, split): columns [split * span, ...) of the row's count in chunks of 8192, each thread 32 of them in 16-byte pieces.
-template <class T>
-__global__ __launch_bounds__(kThreads) void logprobs_kernel(const T* __restrict__ scores, int64_t ld, int n, const int32_t* __restrict__ counts, float scale, float sign,
+template <bool NEG, class T>
+__global__ __launch_bounds__(kThreads) void logprobs_kernel(const T* __restrict__ scores, int64_t ld, int n, const int32_t* __restrict__ counts, float scale,
                                                             const int32_t* __restrict__ targets, int n_targets, int k, int splits, float* __restrict__ logprobs,
                                                             float* __restrict__ logsum, float* __restrict__ entropy, int32_t* __restrict__ ids, float* __restrict__ top_logprobs,
                                                             Stats* __restrict__ part_stats, uint64_t* __restrict__ part_keys) {
@@ -247,7 +284,7 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(const T* __restrict_
     Stats st{-INFINITY, 0.0f, 0.0f, 0};
     TopK tk;
     const int whole = count / kChunk;
-    const T masked = (T)(-sign * INFINITY);
+    const T masked = (T)(NEG ? INFINITY : -INFINITY);
     T next[P][V];          // the next chunk is requested before this one is worked on
     auto fetch = [&](int c) {
         const int64_t base = (int64_t)c * kChunk + threadIdx.x * V;
@@ -269,7 +306,7 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(const T* __restrict_
 #pragma unroll
         for (int p = 0; p < P; p++)
 #pragma unroll
-            for (int i = 0; i < V; i++) v[p * V + i] = signed_score(next[p][i], sign);
+            for (int i = 0; i < V; i++) v[p * V + i] = signed_score<NEG>(next[p][i]);
         if (c + 1 < c_end) fetch(c + 1);
         float top = v[0];
 #pragma unroll
@@ -295,28 +332,46 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(const T* __restrict_
             for (int i = 0; i < kEpt; i++) st.bad |= v[i] != v[i] ? 1 : 0;
         }
         if (k > 0) {
-            const float thr = tk.thr ? unordered((uint32_t)(tk.thr >> 32)) : -INFINITY;      // later columns lose a tie: strictly greater
+            const float thr = tk.thr ? key_score(tk.thr) : -INFINITY;                         // later columns lose a tie: strictly greater
             uint64_t take[kEpt];
             const bool any = __ballot(top > thr) != 0;
 #pragma unroll
             for (int i = 0; i < kEpt; i++) take[i] = any ? __ballot(v[i] > thr) : 0;           // false for NaN and for -inf
-            add_candidates(sh, tk, k, take, [&](int i) { return make_key(v[i], (uint32_t)(base + (i / V) * (kThreads * V) + i % V)); });
+            struct Chunk {
+                const float (&v)[kEpt]; float top, thr; uint32_t base;
+                static constexpr int offset(int i) { return (i / V) * (kThreads * V) + i % V; }
+                __device__ __forceinline__ float score(int i) const { return v[i]; }
+                __device__ __forceinline__ uint32_t col(int i) const { return base + offset(i); }
+                __device__ __forceinline__ uint64_t best() const {
+                    uint32_t at = 0;
+#pragma unroll
+                    for (int i = kEpt - 1; i >= 0; i--) at = v[i] == top ? offset(i) : at;      // the lowest column of the thread's largest score
+                    return top > thr ? make_key(top, base + at) : 0;
+                }
+                __device__ __forceinline__ void keep(uint64_t cut, uint64_t (&take)[kEpt]) const {
+                    const float x = cut ? key_score(cut) : -INFINITY;
+                    const uint32_t c = key_col(cut);
+#pragma unroll
+                    for (int i = 0; i < kEpt; i++) take[i] = __ballot(v[i] > x) | (__ballot(v[i] == x) & __ballot(col(i) <= c) & take[i]);
+                }
+            };
+            add_candidates(sh, tk, k, take, Chunk{v, top, thr, (uint32_t)base});
         }
     }
     if (k > 0 && !tk.sorted) compact(sh, tk, k);
     const int cnt = tk.cnt;
     reduce_stats(sh, st, f);
     if (splits == 1) {
-        finish_row(sh, row, x, count, cnt, targets, n_targets, k, scale, sign, logprobs, logsum, entropy, ids, top_logprobs);
+        finish_row<NEG>(sh, row, x, count, cnt, targets, n_targets, k, scale, logprobs, logsum, entropy, ids, top_logprobs);
     } else {
         if (threadIdx.x == 0) part_stats[blockIdx.x] = sh.row;
-        for (int i = threadIdx.x; i < k; i += kThreads) part_keys[(int64_t)blockIdx.x * k + i] = i < cnt ? sh.buf[i] : 0;
+        for (int i = threadIdx.x; i < k; i += kThreads) part_keys[(int64_t)blockIdx.x * k + i] = i < cnt ? sh.key(i) : 0;
     }
 }
 
 // joins a row's splits
-template <class T>
-__global__ __launch_bounds__(kThreads) void logprobs_join_kernel(const T* __restrict__ scores, int64_t ld, int n, const int32_t* __restrict__ counts, float scale, float sign,
+template <bool NEG, class T>
+__global__ __launch_bounds__(kThreads) void logprobs_join_kernel(const T* __restrict__ scores, int64_t ld, int n, const int32_t* __restrict__ counts, float scale,
                                                                  const int32_t* __restrict__ targets, int n_targets, int k, int splits, float* __restrict__ logprobs,
                                                                  float* __restrict__ logsum, float* __restrict__ entropy, int32_t* __restrict__ ids, float* __restrict__ top_logprobs,
                                                                  const Stats* __restrict__ part_stats, const uint64_t* __restrict__ part_keys) {
@@ -338,12 +393,27 @@ __global__ __launch_bounds__(kThreads) void logprobs_join_kernel(const T* __rest
         for (int i = 0; i < E; i++) { const int at = b + i * kThreads + (int)threadIdx.x; q[i] = at < total ? keys[at] : 0; }
 #pragma unroll
         for (int i = 0; i < E; i++) take[i] = __ballot(q[i] > tk.thr);
-        add_candidates(sh, tk, k, take, [&](int i) { return q[i]; });
+        struct Keys {
+            const uint64_t (&q)[E];
+            __device__ __forceinline__ float score(int i) const { return key_score(q[i]); }
+            __device__ __forceinline__ uint32_t col(int i) const { return key_col(q[i]); }
+            __device__ __forceinline__ uint64_t best() const {
+                uint64_t b = 0;
+#pragma unroll
+                for (int i = 0; i < E; i++) b = q[i] > b ? q[i] : b;
+                return b;
+            }
+            __device__ __forceinline__ void keep(uint64_t cut, uint64_t (&take)[E]) const {
+#pragma unroll
+                for (int i = 0; i < E; i++) take[i] &= __ballot(q[i] >= cut);
+            }
+        };
+        add_candidates(sh, tk, k, take, Keys{q});
     }
     if (k > 0 && !tk.sorted) compact(sh, tk, k);
     const int cnt = tk.cnt;
     reduce_stats(sh, st, f);
-    finish_row(sh, row, scores + row * ld, count, cnt, targets, n_targets, k, scale, sign, logprobs, logsum, entropy, ids, top_logprobs);
+    finish_row<NEG>(sh, row, scores + row * ld, count, cnt, targets, n_targets, k, scale, logprobs, logsum, entropy, ids, top_logprobs);
 }
 
 // Splits of a row: enough workgroups for four per CU, none with less than one chunk.
@@ -353,8 +423,7 @@ int split_count(int64_t m, int64_t n) {
     return (int)std::min(chunks, std::max<int64_t>(1, kGroups / m));
 }
 
-template <class T> void logprobs_t(hipStream_t s, const LogProbsArgs& a) {
-    const float sign = a.scale < 0 ? -1.0f : 1.0f;
+template <bool NEG, class T> void logprobs_t(hipStream_t s, const LogProbsArgs& a) {
     const float scale = std::fabs(a.scale);
     constexpr int64_t kPiece = (int64_t)1 << 24;
     for (int64_t i = 0; i < a.m; i += kPiece) {
@@ -368,11 +437,11 @@ template <class T> void logprobs_t(hipStream_t s, const LogProbsArgs& a) {
         float* lp = a.n_targets ? a.logprobs + i * a.n_targets : nullptr;
         int32_t* ids = a.k ? a.ids + i * a.k : nullptr;
         float* tl = a.k ? a.top_logprobs + i * a.k : nullptr;
-        hipLaunchKernelGGL((logprobs_kernel<T>), dim3((unsigned)(m * splits)), dim3(kThreads), 0, s, x, a.ld, a.n, counts, scale, sign, targets, a.n_targets, a.k, splits,
+        hipLaunchKernelGGL((logprobs_kernel<NEG, T>), dim3((unsigned)(m * splits)), dim3(kThreads), 0, s, x, a.ld, a.n, counts, scale, targets, a.n_targets, a.k, splits,
                            lp, a.logsum + i, a.entropy + i, ids, tl, ps, pk);
         LAUNCH_CHECK();
         if (splits > 1) {
-            hipLaunchKernelGGL((logprobs_join_kernel<T>), dim3((unsigned)m), dim3(kThreads), 0, s, x, a.ld, a.n, counts, scale, sign, targets, a.n_targets, a.k, splits,
+            hipLaunchKernelGGL((logprobs_join_kernel<NEG, T>), dim3((unsigned)m), dim3(kThreads), 0, s, x, a.ld, a.n, counts, scale, targets, a.n_targets, a.k, splits,
                                lp, a.logsum + i, a.entropy + i, ids, tl, ps, pk);
             LAUNCH_CHECK();
         }
@@ -390,9 +459,13 @@ size_t logprobs_work_bytes(int64_t m, int64_t n, int32_t k) {
 
 void launch_logprobs(hipStream_t s, const LogProbsArgs& a) {
     if (a.m <= 0) return;
-    if (a.dtype == COMET_F32) logprobs_t<float>(s, a);
-    else if (a.dtype == COMET_F16) logprobs_t<_Float16>(s, a);
-    else logprobs_t<__bf16>(s, a);
+    auto typed = [&](auto neg) {
+        constexpr bool NEG = decltype(neg)::value;
+        if (a.dtype == COMET_F32) logprobs_t<NEG, float>(s, a);
+        else if (a.dtype == COMET_F16) logprobs_t<NEG, _Float16>(s, a);
+        else logprobs_t<NEG, __bf16>(s, a);
+    };
+    if (a.scale < 0) typed(std::true_type{}); else typed(std::false_type{});
 }
 
 }  // namespace comet
