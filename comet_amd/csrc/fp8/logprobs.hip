@@ -51,7 +51,6 @@ struct Shared {
     uint64_t cut;
     int total[2][kWaves];
     float sm[kWaves], ss[kWaves], sw[kWaves]; int sb[kWaves];
-    Stats row;
 };
 
 struct TopK { int cnt = 0; uint64_t thr = 0; bool sorted = true; int turn = 0; };    // the same in every thread; thr: at least k of the keys so far are not below it (0: unknown)
@@ -224,39 +223,61 @@ __device__ __forceinline__ void add_candidates(Shared& sh, TopK& tk, int k, uint
     if (tk.cnt >= k + kThreads) compact(sh, tk, k);
 }
 
-__device__ void reduce_stats(Shared& sh, Stats st, float f) {
+template <int X = 1, class F> __device__ __forceinline__ float reduce_wave(float v, F join) {      // over the 64 lanes, always in the same order
+    v = join(v, __builtin_bit_cast(float, xor_lane<X>(__builtin_bit_cast(uint32_t, v))));
+    if constexpr (X < 32) return reduce_wave<2 * X>(v, join);
+    else return v;
+}
+
+// a row's statistics from its threads', in every thread
+__device__ Stats reduce_stats(Shared& sh, Stats st, float f) {
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const float wave_max = reduce_wave(st.m, [](float a, float b) { return fmaxf(a, b); });
+    if (lane == 0) sh.sm[wave] = wave_max;
+    __syncthreads();
+    float m = sh.sm[0];
 #pragma unroll
-    for (int o = 1; o < 64; o <<= 1) stats_join(st, __shfl_xor(st.m, o, 64), __shfl_xor(st.s, o, 64), __shfl_xor(st.w, o, 64), __shfl_xor(st.bad, o, 64), f);
-    if (lane == 0) { sh.sm[wave] = st.m; sh.ss[wave] = st.s; sh.sw[wave] = st.w; sh.sb[wave] = st.bad; }
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        Stats a{sh.sm[0], sh.ss[0], sh.sw[0], sh.sb[0]};
-        for (int w = 1; w < kThreads / 64; w++) stats_join(a, sh.sm[w], sh.ss[w], sh.sw[w], sh.sb[w], f);
-        sh.row = a;
+    for (int w = 1; w < kWaves; w++) m = fmaxf(m, sh.sm[w]);
+    float s = 0.0f, w = 0.0f;
+    if (m > -INFINITY) {
+        const float t = (st.m - m) * f, e = exp2_t(t);
+        w = (st.w + fmaxf(t, -1e30f) * st.s) * e;            // -inf * 0 would be NaN; a NaN stays in e
+        s = st.s * e;
     }
+    auto add = [](float a, float b) { return a + b; };
+    s = reduce_wave(s, add); w = reduce_wave(w, add);
+    const uint64_t bad = __ballot(st.bad != 0);
+    if (lane == 0) { sh.ss[wave] = s; sh.sw[wave] = w; sh.sb[wave] = bad != 0; }
     __syncthreads();
+    Stats r{m, 0.0f, 0.0f, 0};
+#pragma unroll
+    for (int i = 0; i < kWaves; i++) { r.s += sh.ss[i]; r.w += sh.sw[i]; r.bad |= sh.sb[i]; }
+    return r;
 }
 
 template <bool NEG, class T> __device__ __forceinline__ float signed_score(T v) { return NEG ? -(float)v : (float)v; }
 
-// a row's outputs from its statistics and its sorted best keys (sh.row, the sorted candidates 0 .. cnt)
+// the score of the thread's first target: requested at the start of a row's last kernel, used at its end
+struct Target { float score; bool in; };
+template <bool NEG, class T> __device__ __forceinline__ Target load_target(const T* x, int count, const int32_t* targets, int t, int n_targets) {
+    const int32_t col = t < n_targets ? targets[t] : -1;
+    const bool in = col >= 0 && col < count;
+    return Target{in ? signed_score<NEG>(x[col]) : 0.0f, in};
+}
+
+// a row's outputs from its statistics and its sorted candidates 0 .. cnt
 template <bool NEG, class T>
-__device__ void finish_row(Shared& sh, int64_t row, const T* x, int count, int cnt, const int32_t* targets, int n_targets, int k, float scale,
-                           float* logprobs, float* logsum, float* entropy, int32_t* ids, float* top_logprobs) {
-    const Stats st = sh.row;
+__device__ __forceinline__ void finish_row(const Shared& sh, const Stats& st, int64_t row, const T* x, int count, int cnt, const int32_t* targets, Target mine, int n_targets, int k,
+                                           float scale, float* logprobs, float* logsum, float* entropy, int32_t* ids, float* top_logprobs) {
     const bool empty = !st.bad && st.m == -INFINITY;
-    const float nan = __builtin_nanf("");
-    const float log_s = st.bad ? nan : logf(st.s);
+    const float log_s = st.bad ? __builtin_nanf("") : logf(st.s);
     if (threadIdx.x == 0) {
         logsum[row] = empty ? -INFINITY : st.m * scale + log_s;
         entropy[row] = empty ? 0.0f : log_s - kLn2 * (st.w / st.s);
     }
     for (int t = threadIdx.x; t < n_targets; t += kThreads) {
-        const int32_t col = targets[row * n_targets + t];
-        float v = -INFINITY;
-        if (!empty && col >= 0 && col < count) v = (signed_score<NEG>(x[col]) - st.m) * scale - log_s;
-        logprobs[row * n_targets + t] = v;
+        if (t >= kThreads) mine = load_target<NEG>(x, count, targets, t, n_targets);
+        logprobs[row * n_targets + t] = !empty && mine.in ? (mine.score - st.m) * scale - log_s : -INFINITY;
     }
     for (int i = threadIdx.x; i < k; i += kThreads) {
         const bool has = i < cnt;
@@ -283,6 +304,9 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(const T* __restrict_
     const float f = scale * kLog2e;
     Stats st{-INFINITY, 0.0f, 0.0f, 0};
     TopK tk;
+    const int32_t* row_targets = targets + row * n_targets;
+    Target target{0.0f, false};
+    if (splits == 1) target = load_target<NEG>(x, count, row_targets, threadIdx.x, n_targets);
     const int whole = count / kChunk;
     const T masked = (T)(NEG ? INFINITY : -INFINITY);
     T next[P][V];          // the next chunk is requested before this one is worked on
@@ -360,11 +384,11 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(const T* __restrict_
     }
     if (k > 0 && !tk.sorted) compact(sh, tk, k);
     const int cnt = tk.cnt;
-    reduce_stats(sh, st, f);
+    st = reduce_stats(sh, st, f);
     if (splits == 1) {
-        finish_row<NEG>(sh, row, x, count, cnt, targets, n_targets, k, scale, logprobs, logsum, entropy, ids, top_logprobs);
+        finish_row<NEG>(sh, st, row, x, count, cnt, row_targets, target, n_targets, k, scale, logprobs, logsum, entropy, ids, top_logprobs);
     } else {
-        if (threadIdx.x == 0) part_stats[blockIdx.x] = sh.row;
+        if (threadIdx.x == 0) part_stats[blockIdx.x] = st;
         for (int i = threadIdx.x; i < k; i += kThreads) part_keys[(int64_t)blockIdx.x * k + i] = i < cnt ? sh.key(i) : 0;
     }
 }
@@ -381,6 +405,9 @@ __global__ __launch_bounds__(kThreads) void logprobs_join_kernel(const T* __rest
     int count = n;
     if (counts) { count = counts[row]; count = count < 0 ? 0 : (count > n ? n : count); }
     const float f = scale * kLog2e;
+    const T* x = scores + row * ld;
+    const int32_t* row_targets = targets + row * n_targets;
+    const Target target = load_target<NEG>(x, count, row_targets, threadIdx.x, n_targets);
     Stats st{-INFINITY, 0.0f, 0.0f, 0};
     for (int i = threadIdx.x; i < splits; i += kThreads) { const Stats p = part_stats[row * splits + i]; stats_join(st, p.m, p.s, p.w, p.bad, f); }
     TopK tk;
@@ -412,8 +439,8 @@ __global__ __launch_bounds__(kThreads) void logprobs_join_kernel(const T* __rest
     }
     if (k > 0 && !tk.sorted) compact(sh, tk, k);
     const int cnt = tk.cnt;
-    reduce_stats(sh, st, f);
-    finish_row<NEG>(sh, row, scores + row * ld, count, cnt, targets, n_targets, k, scale, logprobs, logsum, entropy, ids, top_logprobs);
+    st = reduce_stats(sh, st, f);
+    finish_row<NEG>(sh, st, row, x, count, cnt, row_targets, target, n_targets, k, scale, logprobs, logsum, entropy, ids, top_logprobs);
 }
 
 // Splits of a row: enough workgroups for four per CU, none with less than one chunk.
