@@ -114,117 +114,166 @@ __global__ __launch_bounds__(256) void scores_stream_kernel(const uint8_t* __res
     }
 }
 
-// Many queries: a workgroup takes 128 queries x 128 rows, its four waves 64 x 64 each, and walks the blocks with both operands' codes in two LDS buffers that
-// are filled by the memory pipe itself: while one block is multiplied the next arrives. A tile of codes is 128 rows of eight 16-byte pieces; piece c of row r
-// lies at place c ^ (r & 7), so that the sixteen rows of an operand read fall on all banks (the fill permutes its global addresses, not its LDS ones).
-constexpr int kTile = 128, kTileBytes = kTile * kFp8Block;
+// Many queries: a workgroup of eight waves walks tiles of BM queries x 256 rows, block by block, through a ring of STAGES LDS buffers that the memory pipe
+// fills STAGES - 1 blocks ahead, across tiles: the next tile's first blocks arrive while this one is finished and stored. A wave multiplies QT * 16 queries
+// with RT * 16 rows. One buffer holds the codes of a block (queries, then rows: 128 bytes each) and the rows' and queries' dword of scales. 16-byte piece c
+// of code row r lies at place c ^ (r & 7), so that the sixteen rows of an operand read fall on all banks (the fill permutes its global addresses, not its
+// LDS ones).
+constexpr int kBN = 256, kTileThreads = 512;
+template <int QT, int RT, int WQ> struct TileShape {
+    static constexpr int BM = WQ * QT * 16, rows = BM + kBN, codes = rows * kFp8Block, stage = codes + ((rows * 4 + 2047) / 2048) * 2048;
+    static constexpr int fills = rows / 64 + 1;          // fill instructions a wave issues per block: 8 code rows each, and one for scales
+    static_assert((8 / WQ) * RT * 16 == kBN && rows % 64 == 0 && rows <= kTileThreads, "eight waves cover the tile");
+};
 
-// The fill is an asm statement: around the compiler's own form of it every LDS read that follows would wait for the fill just issued (it cannot tell the two
-// buffers apart). The waits are written out where the buffers change hands. It has no register outputs; M0 holds the LDS address of the wave's 1 KiB.
-__device__ __forceinline__ void fill_1k(const uint8_t* base /* uniform */, uint32_t offset, uint32_t lds /* uniform */) {
+// The fills are asm statements: around the compiler's own form of them every LDS read that follows would wait for the fill just issued (it cannot tell the
+// buffers apart). The waits are written out where a buffer changes hands. No register outputs; M0 holds the LDS address of the wave's part.
+__device__ __forceinline__ void fill16(const uint8_t* base /* uniform */, uint32_t offset, uint32_t lds /* uniform */) {
     const uint64_t b = (uint64_t)base;
     const uint64_t sb = ((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(b >> 32)) << 32) | (uint32_t)__builtin_amdgcn_readfirstlane((int)b);
     asm volatile("s_mov_b32 m0, %2\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %0, %1" :: "v"(offset), "s"(sb), "s"(__builtin_amdgcn_readfirstlane((int)lds)) : "memory");
 }
-// A wave's eighth-of-eight rows of a tile: instruction i fills rows (4 i + wave) * 8 .. + 7. offset[i]: the lane's 16 bytes relative to the tile's first row
-// (rows past the matrix's last read the last one).
-__device__ __forceinline__ void tile_offsets(int64_t first, int64_t count, int64_t row_bytes, uint32_t (&offset)[4]) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        int64_t r = (i * 4 + wave) * 8 + (lane >> 3);
-        r = first + r < count ? r : count - 1 - first;
-        offset[i] = (uint32_t)(r * row_bytes) + ((lane & 7) ^ (lane >> 3)) * 16;
-    }
-}
-__device__ __forceinline__ void fill_tile(const uint8_t* base, const uint32_t (&offset)[4], uint32_t lds) {
-    const int wave = threadIdx.x >> 6;
-#pragma unroll
-    for (int i = 0; i < 4; i++) fill_1k(base, offset[i], lds + (i * 4 + wave) * 1024);
+__device__ __forceinline__ void fill4(const uint8_t* address, uint32_t lds /* uniform */) {
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 3\n\tglobal_load_lds_dword %0, off" :: "v"(address), "s"(__builtin_amdgcn_readfirstlane((int)lds)) : "memory");
 }
 __device__ __forceinline__ uint32_t lds_address(const void* p) { return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)p; }
-// a lane's two pieces of tile row r0 + lane % 16
-__device__ __forceinline__ v8i read_tile(const uint8_t* lds, int r0) {
-    const int lane = threadIdx.x & 63, r = r0 + (lane & 15), g = lane >> 4;
-    const uint8_t* p = lds + r * kFp8Block;
-    const v4i a = *(const v4i*)(p + ((g ^ (r & 7)) * 16)), b = *(const v4i*)(p + (((4 + g) ^ (r & 7)) * 16));
-    return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
-}
+template <int N> __device__ __forceinline__ void wait_vm() { asm volatile("s_waitcnt vmcnt(%0)" :: "n"(N) : "memory"); }
 
-template <class T>
-__global__ __launch_bounds__(256, 2) void scores_tile_kernel(const uint8_t* __restrict__ qc, const uint8_t* __restrict__ qs, int m, const uint8_t* __restrict__ rc,
-                                                             const uint8_t* __restrict__ rs, int n, int nb, int nb4, T* __restrict__ out, int64_t ld, int m_tiles, int n_tiles) {
-    __shared__ __align__(16) uint8_t lds[2][2][kTileBytes];
-    // Workgroups go to the eight XCDs in turn; each XCD takes a contiguous run of the tiles, queries fastest, so that a row tile is read into one L2.
-    const int tiles = m_tiles * n_tiles, per = (tiles + 7) / 8;
-    const int tile = (int)(blockIdx.x & 7) * per + (int)(blockIdx.x >> 3);
-    if (tile >= tiles) return;
-    const int64_t m0 = (int64_t)(tile % m_tiles) * kTile, n0 = (int64_t)(tile / m_tiles) * kTile;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int wm = (wave & 1) * 64, wn = (wave >> 1) * 64;
+template <class T, int QT, int RT, int WQ, int STAGES>
+__global__ __launch_bounds__(kTileThreads, 2) void scores_tile_kernel(const uint8_t* __restrict__ qc, const uint8_t* __restrict__ qs, int m, const uint8_t* __restrict__ rc,
+                                                                      const uint8_t* __restrict__ rs, int n, int nb, int nb4, T* __restrict__ out, int64_t ld, int m_tiles, int n_tiles) {
+    using Shape = TileShape<QT, RT, WQ>;
+    extern __shared__ __align__(16) uint8_t lds[];
+    constexpr int BM = Shape::BM, F = Shape::fills, ST = QT * RT;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wq = (wave % WQ) * QT * 16, wr = (wave / WQ) * RT * 16;
     const int64_t row_bytes = (int64_t)nb * kFp8Block;
-    const uint8_t *qsp[4], *rsp[4];
+    // Workgroups go to the eight XCDs in turn; each XCD takes a contiguous run of the tiles, queries fastest, dealt to its workgroups in turn: a row tile is
+    // read into one L2, by neighbours at about the same time.
+    const int tiles = m_tiles * n_tiles, per = (tiles + 7) / 8, xcd = (int)(blockIdx.x & 7), groups = (int)(gridDim.x >> 3);
+    const int t0 = xcd * per + (int)(blockIdx.x >> 3), t_end = min(tiles, (xcd + 1) * per);
+    if (t0 >= t_end) return;
+    const int steps = ((t_end - t0 - 1) / groups + 1) * nb;
+    const uint32_t l0 = lds_address(lds);
+
+    // the tile being filled: a lane's byte offsets from the first query / row, and its scale dword's address
+    constexpr int FQ = BM / 64, FR = kBN / 64;
+    int f_tile = t0, f_b = 0, f_stage = 0;
+    const uint8_t *fq_base = nullptr, *fr_base = nullptr, *f_scale = nullptr;
+    uint32_t fq[FQ], fr[FR];
+    auto fill_tile = [&] {
+        const int64_t m0 = (int64_t)(f_tile % m_tiles) * BM, n0 = (int64_t)(f_tile / m_tiles) * kBN;
+        fq_base = qc + m0 * row_bytes; fr_base = rc + n0 * row_bytes;
+        const uint32_t piece = ((lane & 7) ^ (lane >> 3)) * 16;
+        const int last_q = (int)min((int64_t)BM, m - m0) - 1, last_r = (int)min((int64_t)kBN, n - n0) - 1;       // rows past the end read the last one: their products go nowhere
 #pragma unroll
-    for (int t = 0; t < 4; t++) {
-        int64_t q = m0 + wm + t * 16 + (lane & 15), r = n0 + wn + t * 16 + (lane & 15);
-        qsp[t] = qs + (q < m ? q : m - 1) * nb4; rsp[t] = rs + (r < n ? r : n - 1) * nb4;
-    }
-    v4f acc[4][4];
+        for (int i = 0; i < FQ; i++) fq[i] = (uint32_t)(min((i * 8 + wave) * 8 + (lane >> 3), last_q) * row_bytes) + piece;
 #pragma unroll
-    for (int t = 0; t < 4; t++)
+        for (int i = 0; i < FR; i++) fr[i] = (uint32_t)(min((i * 8 + wave) * 8 + (lane >> 3), last_r) * row_bytes) + piece;
+        const int r = (int)threadIdx.x;
+        f_scale = r < BM ? qs + (m0 + min(r, last_q)) * nb4 : rs + (n0 + min(r - BM, last_r)) * nb4;
+    };
+    auto fill = [&] {
+        const uint32_t to = l0 + f_stage * Shape::stage;
 #pragma unroll
-        for (int v = 0; v < 4; v++) acc[t][v] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-    uint32_t qo[4], ro[4];
-    tile_offsets(m0, m, row_bytes, qo); tile_offsets(n0, n, row_bytes, ro);
-    const uint8_t *qb0 = qc + m0 * row_bytes, *rb0 = rc + n0 * row_bytes;
-    const uint32_t l0 = lds_address(&lds[0][0][0]);
-    uint32_t sr[4], sq[4], sr_next[4], sq_next[4];
+        for (int i = 0; i < FQ; i++) fill16(fq_base + f_b * kFp8Block, fq[i], to + (i * 8 + wave) * 1024);
 #pragma unroll
-    for (int t = 0; t < 4; t++) { sr_next[t] = *(const uint32_t*)rsp[t]; sq_next[t] = *(const uint32_t*)qsp[t]; }
-    fill_tile(qb0, qo, l0); fill_tile(rb0, ro, l0 + kTileBytes);
-    for (int b = 0; b < nb; b++) {
-        // this block and its scales have arrived for every wave, and every wave is done with the buffer that the next one goes to
-        asm volatile("s_waitcnt vmcnt(0)" : "+v"(sr_next[0]), "+v"(sr_next[1]), "+v"(sr_next[2]), "+v"(sr_next[3]), "+v"(sq_next[0]), "+v"(sq_next[1]), "+v"(sq_next[2]), "+v"(sq_next[3]) :: "memory");
-        __builtin_amdgcn_s_barrier();
+        for (int i = 0; i < FR; i++) fill16(fr_base + f_b * kFp8Block, fr[i], to + BM * kFp8Block + (i * 8 + wave) * 1024);
+        fill4(f_scale + (f_b & ~3), to + Shape::codes + wave * 256);
+        f_stage = f_stage + 1 == STAGES ? 0 : f_stage + 1;
+        if (++f_b == nb) { f_b = 0; f_tile += groups; if (f_tile < t_end) fill_tile(); }
+    };
+    fill_tile();
+#pragma unroll
+    for (int i = 0; i < STAGES - 1; i++) if (i < steps) fill();
+
+    v4f acc[RT][QT];
+#pragma unroll
+    for (int t = 0; t < RT; t++)
+#pragma unroll
+        for (int v = 0; v < QT; v++) acc[t][v] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+    int tile = t0, b = 0, stage = 0;
+    int stored = STAGES;            // steps since the last full tile was stored
+    for (int step = 0; step < steps; step++) {
+        // Block `step` has arrived when only what was issued behind its fill is left: the fills of the STAGES - 2 blocks after it and one tile's stores (ST per
+        // wave when the tile lay inside the matrix), if they came since. At the end, where fewer fills follow, everything is waited for.
+        if (step + STAGES - 2 >= steps) wait_vm<0>();
+        else if (stored < STAGES - 1) wait_vm<(STAGES - 2) * F + ST>();
+        else wait_vm<(STAGES - 2) * F>();
+        __builtin_amdgcn_s_barrier();       // ... for every wave, and every wave is done with the buffer that is filled next
         asm volatile("" ::: "memory");
-        if ((b & 3) == 0) {
+        if (step + STAGES - 1 < steps) fill();
+        const uint8_t* buf = lds + stage * Shape::stage;
+        float sr[RT], sq[QT];
 #pragma unroll
-            for (int t = 0; t < 4; t++) { sr[t] = sr_next[t]; sq[t] = sq_next[t]; }
-        }
-        if (b + 1 < nb) {
-            const uint32_t to = l0 + ((b + 1) & 1) * (2 * kTileBytes);
-            fill_tile(qb0 + (b + 1) * kFp8Block, qo, to); fill_tile(rb0 + (b + 1) * kFp8Block, ro, to + kTileBytes);
-            if (((b + 1) & 3) == 0) {
+        for (int t = 0; t < RT; t++) sr[t] = __builtin_bit_cast(float, (uint32_t)buf[Shape::codes + (BM + wr + t * 16 + (lane & 15)) * 4 + (b & 3)] << 23);
 #pragma unroll
-                for (int t = 0; t < 4; t++) { sr_next[t] = *(const uint32_t*)(rsp[t] + b + 1); sq_next[t] = *(const uint32_t*)(qsp[t] + b + 1); }
+        for (int v = 0; v < QT; v++) sq[v] = __builtin_bit_cast(float, (uint32_t)buf[Shape::codes + (wq + v * 16 + (lane & 15)) * 4 + (b & 3)] << 23);
+#pragma unroll
+        for (int h = 0; h < 2; h++) {       // the lane's two 16-byte pieces of each row
+            auto piece = [&](int r) { return *(const v4i*)(buf + r * kFp8Block + ((((lane >> 4) + 4 * h) ^ (r & 7)) * 16)); };
+            v4i r[RT], q[QT];
+#pragma unroll
+            for (int t = 0; t < RT; t++) r[t] = piece(BM + wr + t * 16 + (lane & 15));
+#pragma unroll
+            for (int v = 0; v < QT; v++) q[v] = piece(wq + v * 16 + (lane & 15));
+#pragma unroll
+            for (int w = 0; w < 2; w++) {
+                v8b rb[RT];
+#pragma unroll
+                for (int t = 0; t < RT; t++) rb[t] = widen(r[t][2 * w], r[t][2 * w + 1], sr[t]);
+#pragma unroll
+                for (int v = 0; v < QT; v++) {
+                    const v8b qb = widen(q[v][2 * w], q[v][2 * w + 1], sq[v]);
+#pragma unroll
+                    for (int t = 0; t < RT; t++) acc[t][v] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(rb[t], qb, acc[t][v], 0, 0, 0);
+                }
             }
         }
-        const uint8_t *lq = lds[b & 1][0], *lr = lds[b & 1][1];
-        v8i r[4], q[4];
-        float fr[4], fq[4];
+        stage = stage + 1 == STAGES ? 0 : stage + 1;
+        stored++;
+        if (++b == nb) {
+            const int64_t m0 = (int64_t)(tile % m_tiles) * BM, n0 = (int64_t)(tile / m_tiles) * kBN;
+            T* to = out + (m0 + wq + (lane & 15)) * ld + n0 + wr + (lane >> 4) * 4;
+            if (m0 + BM <= m && n0 + kBN <= n) {
 #pragma unroll
-        for (int t = 0; t < 4; t++) {
-            r[t] = read_tile(lr, wn + t * 16); q[t] = read_tile(lq, wm + t * 16);
-            fr[t] = scale_of(sr[t], b & 3); fq[t] = scale_of(sq[t], b & 3);
-        }
+                for (int v = 0; v < QT; v++)
 #pragma unroll
-        for (int w = 0; w < 4; w++) {
-            v8b qb[4], rb[4];
+                    for (int t = 0; t < RT; t++) {
+                        T o[4];
 #pragma unroll
-            for (int t = 0; t < 4; t++) { qb[t] = widen(q[t][2 * w], q[t][2 * w + 1], fq[t]); rb[t] = widen(r[t][2 * w], r[t][2 * w + 1], fr[t]); }
+                        for (int i = 0; i < 4; i++) o[i] = (T)acc[t][v][i];
+                        __builtin_memcpy(to + v * 16 * ld + t * 16, o, sizeof(o));
+                    }
+                stored = 0;
+            } else {
 #pragma unroll
-            for (int t = 0; t < 4; t++)
+                for (int v = 0; v < QT; v++) {
+                    const int64_t q = m0 + wq + v * 16 + (lane & 15);
+                    if (q >= m) continue;
 #pragma unroll
-                for (int v = 0; v < 4; v++) acc[t][v] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(rb[t], qb[v], acc[t][v], 0, 0, 0);
+                    for (int t = 0; t < RT; t++) store4(out + q * ld, n0 + wr + t * 16 + (lane >> 4) * 4, n, acc[t][v]);
+                }
+            }
+#pragma unroll
+            for (int t = 0; t < RT; t++)
+#pragma unroll
+                for (int v = 0; v < QT; v++) acc[t][v] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+            b = 0; tile += groups;
         }
     }
-#pragma unroll
-    for (int v = 0; v < 4; v++) {
-        const int64_t q = m0 + wm + v * 16 + (lane & 15);
-        if (q >= m) continue;
-#pragma unroll
-        for (int t = 0; t < 4; t++) store4(out + q * ld, n0 + wn + t * 16 + (lane >> 4) * 4, n, acc[t][v]);
-    }
+}
+
+template <class T, int QT, int RT, int WQ, int STAGES>
+void launch_tiles(hipStream_t s, const uint8_t* qc, const uint8_t* qs, int m, const uint8_t* rc, const uint8_t* rs, int n, int nb, int nb4, T* out, int64_t ld) {
+    using Shape = TileShape<QT, RT, WQ>;
+    constexpr int bytes = STAGES * Shape::stage;
+    static_assert(bytes <= 160 * 1024, "LDS of a CU");
+    auto kernel = scores_tile_kernel<T, QT, RT, WQ, STAGES>;
+    HIP_CHECK(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    const int mt = (int)ceil_div(m, Shape::BM), nt = (int)ceil_div(n, kBN);
+    const int64_t groups = std::min<int64_t>(256, round_up((int64_t)mt * nt, 8));      // one workgroup per CU
+    hipLaunchKernelGGL(kernel, dim3((unsigned)groups), dim3(kTileThreads), bytes, s, qc, qs, m, rc, rs, n, nb, nb4, out, ld, mt, nt);
 }
 
 template <class T> void scores_t(hipStream_t s, const Fp8View& q, int64_t q_first, int64_t m, const Fp8View& r, int64_t first, int64_t n, T* out, int64_t ld) {
@@ -236,10 +285,8 @@ template <class T> void scores_t(hipStream_t s, const Fp8View& q, int64_t q_firs
         T* o = out + i * ld + j;
         const int64_t nt = ceil_div(nj, 256);
         if (mi <= 16) hipLaunchKernelGGL((scores_stream_kernel<T, 1>), dim3((unsigned)nt), dim3(256), 0, s, qc, qs, mi, rc, rs, nj, r.nb, r.nb4, o, ld, 1);
-        else {
-            const int mt = (int)ceil_div(mi, kTile), ntile = (int)ceil_div(nj, kTile);
-            hipLaunchKernelGGL((scores_tile_kernel<T>), dim3((unsigned)(ceil_div((int64_t)mt * ntile, 8) * 8)), dim3(256), 0, s, qc, qs, mi, rc, rs, nj, r.nb, r.nb4, o, ld, mt, ntile);
-        }
+        else if (mi > 128) launch_tiles<T, 8, 4, 2, 2>(s, qc, qs, mi, rc, rs, nj, r.nb, r.nb4, o, ld);
+        else launch_tiles<T, 4, 4, 2, 3>(s, qc, qs, mi, rc, rs, nj, r.nb, r.nb4, o, ld);
         LAUNCH_CHECK();
     }
 }
