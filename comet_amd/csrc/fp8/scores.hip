@@ -118,16 +118,15 @@ __global__ __launch_bounds__(256) void scores_stream_kernel(const uint8_t* __res
         }
 }
 
-// Many queries: a workgroup of eight waves walks tiles of BM queries x 256 rows, block by block, through a ring of STAGES LDS buffers that the memory pipe
+// More queries: a workgroup of WAVES waves walks tiles of BM queries x BN rows, block by block, through a ring of STAGES LDS buffers that the memory pipe
 // fills STAGES - 1 blocks ahead, across tiles: the next tile's first blocks arrive while this one is finished and stored. A wave multiplies QT * 16 queries
-// with RT * 16 rows. One buffer holds the codes of a block (queries, then rows: 128 bytes each) and the rows' and queries' dword of scales. 16-byte piece c
+// with 64 rows. One buffer holds the codes of a block (queries, then rows: 128 bytes each) and the rows' and queries' dword of scales. 16-byte piece c
 // of code row r lies at place c ^ (r & 7), so that the sixteen rows of an operand read fall on all banks (the fill permutes its global addresses, not its
 // LDS ones).
-constexpr int kBN = 256, kTileThreads = 512;
-template <int QT, int RT, int WQ> struct TileShape {
-    static constexpr int BM = WQ * QT * 16, rows = BM + kBN, codes = rows * kFp8Block, stage = codes + ((rows * 4 + 2047) / 2048) * 2048;
-    static constexpr int fills = rows / 64 + 1;          // fill instructions a wave issues per block: 8 code rows each, and one for scales
-    static_assert((8 / WQ) * RT * 16 == kBN && RT == 4 && rows % 64 == 0 && rows <= kTileThreads, "eight waves cover the tile");
+template <int QT, int WQ, int WAVES> struct TileShape {
+    static constexpr int BM = WQ * QT * 16, BN = WAVES / WQ * 64, rows = BM + BN, codes = rows * kFp8Block, stage = codes + WAVES * 256;
+    static constexpr int FQ = BM / (8 * WAVES), FR = BN / (8 * WAVES), fills = FQ + FR + 1;      // fill instructions a wave issues per block: 8 code rows each, and one for scales
+    static_assert(BM % (8 * WAVES) == 0 && BN % (8 * WAVES) == 0 && rows <= WAVES * 64, "the waves share the fills evenly");
 };
 
 // The fills are asm statements: around the compiler's own form of them every LDS read that follows would wait for the fill just issued (it cannot tell the
@@ -143,12 +142,12 @@ __device__ __forceinline__ void fill4(const uint8_t* address, uint32_t lds /* un
 __device__ __forceinline__ uint32_t lds_address(const void* p) { return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)p; }
 template <int N> __device__ __forceinline__ void wait_vm() { asm volatile("s_waitcnt vmcnt(%0)" :: "n"(N) : "memory"); }
 
-template <class T, int QT, int RT, int WQ, int STAGES>
-__global__ __launch_bounds__(kTileThreads, 2) void scores_tile_kernel(const uint8_t* __restrict__ qc, const uint8_t* __restrict__ qs, int m, const uint8_t* __restrict__ rc,
+template <class T, int QT, int WQ, int WAVES, int STAGES>
+__global__ __launch_bounds__(WAVES * 64, 2) void scores_tile_kernel(const uint8_t* __restrict__ qc, const uint8_t* __restrict__ qs, int m, const uint8_t* __restrict__ rc,
                                                                       const uint8_t* __restrict__ rs, int n, int nb, int nb4, T* __restrict__ out, int64_t ld, int m_tiles, int n_tiles) {
-    using Shape = TileShape<QT, RT, WQ>;
+    using Shape = TileShape<QT, WQ, WAVES>;
     extern __shared__ __align__(16) uint8_t lds[];
-    constexpr int BM = Shape::BM, F = Shape::fills, ST = QT * 4;
+    constexpr int RT = 4, BM = Shape::BM, BN = Shape::BN, FQ = Shape::FQ, FR = Shape::FR, F = Shape::fills, ST = QT * 4;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wq = (wave % WQ) * QT * 16, wr = (wave / WQ) * RT * 16;
     const int64_t row_bytes = (int64_t)nb * kFp8Block;
@@ -161,29 +160,28 @@ __global__ __launch_bounds__(kTileThreads, 2) void scores_tile_kernel(const uint
     const uint32_t l0 = lds_address(lds);
 
     // the tile being filled: a lane's byte offsets from the first query / row, and its scale dword's address
-    constexpr int FQ = BM / 64, FR = kBN / 64;
     int f_tile = t0, f_b = 0, f_stage = 0;
     const uint8_t *fq_base = nullptr, *fr_base = nullptr, *f_scale = nullptr;
     uint32_t fq[FQ], fr[FR];
     auto row_at = [](int place) { return (place & ~63) + (place & 15) * 4 + ((place >> 4) & 3); };
     auto fill_tile = [&] {
-        const int64_t m0 = (int64_t)(f_tile % m_tiles) * BM, n0 = (int64_t)(f_tile / m_tiles) * kBN;
+        const int64_t m0 = (int64_t)(f_tile % m_tiles) * BM, n0 = (int64_t)(f_tile / m_tiles) * BN;
         fq_base = qc + m0 * row_bytes; fr_base = rc + n0 * row_bytes;
         const uint32_t piece = ((lane & 7) ^ (lane >> 3)) * 16;
-        const int last_q = (int)min((int64_t)BM, m - m0) - 1, last_r = (int)min((int64_t)kBN, n - n0) - 1;       // rows past the end read the last one: their products go nowhere
+        const int last_q = (int)min((int64_t)BM, m - m0) - 1, last_r = (int)min((int64_t)BN, n - n0) - 1;       // rows past the end read the last one: their products go nowhere
 #pragma unroll
-        for (int i = 0; i < FQ; i++) fq[i] = (uint32_t)(min((i * 8 + wave) * 8 + (lane >> 3), last_q) * row_bytes) + piece;
+        for (int i = 0; i < FQ; i++) fq[i] = (uint32_t)(min((i * WAVES + wave) * 8 + (lane >> 3), last_q) * row_bytes) + piece;
 #pragma unroll
-        for (int i = 0; i < FR; i++) fr[i] = (uint32_t)(min(row_at((i * 8 + wave) * 8 + (lane >> 3)), last_r) * row_bytes) + piece;
+        for (int i = 0; i < FR; i++) fr[i] = (uint32_t)(min(row_at((i * WAVES + wave) * 8 + (lane >> 3)), last_r) * row_bytes) + piece;
         const int r = (int)threadIdx.x;
         f_scale = r < BM ? qs + (m0 + min(r, last_q)) * nb4 : rs + (n0 + min(row_at(r - BM), last_r)) * nb4;
     };
     auto fill = [&] {
         const uint32_t to = l0 + f_stage * Shape::stage;
 #pragma unroll
-        for (int i = 0; i < FQ; i++) fill16(fq_base + f_b * kFp8Block, fq[i], to + (i * 8 + wave) * 1024);
+        for (int i = 0; i < FQ; i++) fill16(fq_base + f_b * kFp8Block, fq[i], to + (i * WAVES + wave) * 1024);
 #pragma unroll
-        for (int i = 0; i < FR; i++) fill16(fr_base + f_b * kFp8Block, fr[i], to + BM * kFp8Block + (i * 8 + wave) * 1024);
+        for (int i = 0; i < FR; i++) fill16(fr_base + f_b * kFp8Block, fr[i], to + BM * kFp8Block + (i * WAVES + wave) * 1024);
         fill4(f_scale + (f_b & ~3), to + Shape::codes + wave * 256);
         f_stage = f_stage + 1 == STAGES ? 0 : f_stage + 1;
         if (++f_b == nb) { f_b = 0; f_tile += groups; if (f_tile < t_end) fill_tile(); }
@@ -238,9 +236,9 @@ __global__ __launch_bounds__(kTileThreads, 2) void scores_tile_kernel(const uint
         stage = stage + 1 == STAGES ? 0 : stage + 1;
         stored++;
         if (++b == nb) {
-            const int64_t m0 = (int64_t)(tile % m_tiles) * BM, n0 = (int64_t)(tile / m_tiles) * kBN;
+            const int64_t m0 = (int64_t)(tile % m_tiles) * BM, n0 = (int64_t)(tile / m_tiles) * BN;
             const int64_t q0 = m0 + wq + (lane >> 4) * 4, j = n0 + wr + (lane & 15) * 4;
-            if (m0 + BM <= m && n0 + kBN <= n) {
+            if (m0 + BM <= m && n0 + BN <= n) {
                 T* to = out + q0 * ld + j;
 #pragma unroll
                 for (int v = 0; v < QT; v++)
@@ -270,16 +268,27 @@ __global__ __launch_bounds__(kTileThreads, 2) void scores_tile_kernel(const uint
     }
 }
 
-template <class T, int QT, int RT, int WQ, int STAGES>
+template <class T, int QT, int WQ, int WAVES, int STAGES>
 void launch_tiles(hipStream_t s, const uint8_t* qc, const uint8_t* qs, int m, const uint8_t* rc, const uint8_t* rs, int n, int nb, int nb4, T* out, int64_t ld) {
-    using Shape = TileShape<QT, RT, WQ>;
-    constexpr int bytes = STAGES * Shape::stage;
-    static_assert(bytes <= 160 * 1024, "LDS of a CU");
-    auto kernel = scores_tile_kernel<T, QT, RT, WQ, STAGES>;
+    using Shape = TileShape<QT, WQ, WAVES>;
+    constexpr int bytes = STAGES * Shape::stage, per_cu = 8 / WAVES;      // two waves a SIMD
+    static_assert(bytes * per_cu <= 160 * 1024, "LDS of a CU");
+    auto kernel = scores_tile_kernel<T, QT, WQ, WAVES, STAGES>;
     HIP_CHECK(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
-    const int mt = (int)ceil_div(m, Shape::BM), nt = (int)ceil_div(n, kBN);
-    const int64_t groups = std::min<int64_t>(256, round_up((int64_t)mt * nt, 8));      // one workgroup per CU
-    hipLaunchKernelGGL(kernel, dim3((unsigned)groups), dim3(kTileThreads), bytes, s, qc, qs, m, rc, rs, n, nb, nb4, out, ld, mt, nt);
+    const int mt = (int)ceil_div(m, Shape::BM), nt = (int)ceil_div(n, Shape::BN);
+    const int64_t groups = std::min<int64_t>(256 * per_cu, round_up((int64_t)mt * nt, 8));
+    hipLaunchKernelGGL(kernel, dim3((unsigned)groups), dim3(WAVES * 64), bytes, s, qc, qs, m, rc, rs, n, nb, nb4, out, ld, mt, nt);
+}
+
+// Which tile: the fewest rounds of the chip (256 tiles of 256 x 256, 512 of the smaller ones, two a CU), each weighted with its measured time: a round of the
+// large tiles 1, of 128 x 128 0.56, of 64 x 128 0.38. The large ones spend least on LDS reads and conversions for a product (256 x 1M x 768: 414 us, against
+// 471 and 618), the small ones leave less of the chip idle when there are few (2048 x 2048 x 2048: 33 us, against 35 and 58) and waste least on few queries
+// (64 x 1M x 768: 210 us, against 228 and 352).
+enum class Tile { large, middle, small };
+Tile pick_tile(int64_t m, int64_t n) {
+    auto rounds = [&](int64_t bm, int64_t bn, int64_t fit) { return (double)ceil_div(ceil_div(m, bm) * ceil_div(n, bn), fit); };
+    const double large = rounds(256, 256, 256), middle = 0.56 * rounds(128, 128, 512), small = 0.38 * rounds(64, 128, 512);
+    return small <= middle && small <= large ? Tile::small : middle <= large ? Tile::middle : Tile::large;
 }
 
 template <class T> void scores_t(hipStream_t s, const Fp8View& q, int64_t q_first, int64_t m, const Fp8View& r, int64_t first, int64_t n, T* out, int64_t ld) {
@@ -291,8 +300,11 @@ template <class T> void scores_t(hipStream_t s, const Fp8View& q, int64_t q_firs
         T* o = out + i * ld + j;
         const int64_t nt = ceil_div(nj, 256);
         if (mi <= 16) hipLaunchKernelGGL((scores_stream_kernel<T, 1>), dim3((unsigned)nt), dim3(256), 0, s, qc, qs, mi, rc, rs, nj, r.nb, r.nb4, o, ld, 1);
-        else if (mi > 128) launch_tiles<T, 8, 4, 2, 2>(s, qc, qs, mi, rc, rs, nj, r.nb, r.nb4, o, ld);
-        else launch_tiles<T, 4, 4, 2, 3>(s, qc, qs, mi, rc, rs, nj, r.nb, r.nb4, o, ld);
+        else switch (pick_tile(mi, nj)) {
+            case Tile::large: launch_tiles<T, 8, 2, 8, 2>(s, qc, qs, mi, rc, rs, nj, r.nb, r.nb4, o, ld); break;
+            case Tile::middle: launch_tiles<T, 4, 2, 4, 2>(s, qc, qs, mi, rc, rs, nj, r.nb, r.nb4, o, ld); break;
+            case Tile::small: launch_tiles<T, 2, 2, 4, 2>(s, qc, qs, mi, rc, rs, nj, r.nb, r.nb4, o, ld); break;
+        }
         LAUNCH_CHECK();
     }
 }
