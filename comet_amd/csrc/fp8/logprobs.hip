@@ -9,6 +9,7 @@
 // A key is (score, column) in 64 bits, larger is better, equal scores to the lower column; keys are unique, so the result does not depend on the order in
 // which candidates arrive. Candidates wait as the score's own bits over the column's complement and become keys when they are sorted. Bound by reading the scores once.
 #include "fp8.hpp"
+#include "lanes.hpp"
 
 namespace comet {
 namespace {
@@ -55,18 +56,6 @@ struct Shared {
 
 struct TopK { int cnt = 0; uint64_t thr = 0; bool sorted = true; int turn = 0; };    // the same in every thread; thr: at least k of the keys so far are not below it (0: unknown)
 
-// the value of lane ^ X
-template <int X> __device__ __forceinline__ uint32_t xor_lane(uint32_t v) {
-    auto dpp = [](uint32_t x, auto ctrl) { return (uint32_t)__builtin_amdgcn_mov_dpp((int)x, decltype(ctrl)::value, 0xF, 0xF, true); };
-    if constexpr (X == 1) return dpp(v, std::integral_constant<int, 0xB1>{});                                                            // quads: 1 0 3 2
-    else if constexpr (X == 2) return dpp(v, std::integral_constant<int, 0x4E>{});                                                       // quads: 2 3 0 1
-    else if constexpr (X == 4) return dpp(dpp(v, std::integral_constant<int, 0x141>{}), std::integral_constant<int, 0x1B>{});            // eights mirrored, then quads
-    else if constexpr (X == 8) return dpp(v, std::integral_constant<int, 0x128>{});                                                      // sixteens turned by eight
-    else {
-        const auto r = X == 16 ? __builtin_amdgcn_permlane16_swap(v, v, false, false) : __builtin_amdgcn_permlane32_swap(v, v, false, false);
-        return (threadIdx.x & X) ? r[0] : r[1];
-    }
-}
 template <int X> __device__ __forceinline__ uint64_t xor_lane64(uint64_t v) { return ((uint64_t)xor_lane<X>((uint32_t)(v >> 32)) << 32) | xor_lane<X>((uint32_t)v); }
 
 // Sorts N * 256 keys descending, key i * 256 + thread in key[i] of that thread: a bitonic network whose strides below 64 are lane exchanges and whose strides
