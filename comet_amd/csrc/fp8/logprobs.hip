@@ -152,12 +152,14 @@ __device__ void compact(Shared& sh, TopK& tk, int k) {
     if (cnt >= k) tk.thr = sh.key(k - 1);
 }
 
-// Where the wave's candidates go: `take[i]` holds the lanes whose element i is one. Returns the workgroup's number of candidates, `before` those of the lower waves.
-template <int EPT> __device__ __forceinline__ int count_candidates(Shared& sh, TopK& tk, const uint64_t (&take)[EPT], int& before) {
+// Where the wave's candidates go: `take[i]` holds the lanes whose element i is one, `any` says that the wave has one. Returns the workgroup's number of candidates, `before` those of the lower waves.
+template <int EPT> __device__ __forceinline__ int count_candidates(Shared& sh, TopK& tk, bool any, const uint64_t (&take)[EPT], int& before) {
     const int wave = threadIdx.x >> 6;
     int mine = 0;
+    if (any) {
 #pragma unroll
-    for (int i = 0; i < EPT; i++) mine += __popcll(take[i]);
+        for (int i = 0; i < EPT; i++) mine += __popcll(take[i]);
+    }
     int* total = sh.total[tk.turn ^= 1];          // two in turn: the other's readers have passed this barrier before it is written again
     if ((threadIdx.x & 63) == 0) total[wave] = mine;
     __syncthreads();
@@ -171,9 +173,9 @@ template <int EPT> __device__ __forceinline__ int count_candidates(Shared& sh, T
 // Adds this chunk's candidates: take[i] holds the lanes whose element i is one (uniform across the wave). Of `chunk`: best() is the thread's largest key (0:
 // none), keep(cut, take) drops what lies below cut, score(i) and col(i) are an element.
 template <int EPT, class Chunk>
-__device__ __forceinline__ void add_candidates(Shared& sh, TopK& tk, int k, uint64_t (&take)[EPT], const Chunk& chunk) {
+__device__ __forceinline__ void add_candidates(Shared& sh, TopK& tk, int k, bool any, uint64_t (&take)[EPT], const Chunk& chunk) {
     const int lane = threadIdx.x & 63;
-    int before, c = count_candidates(sh, tk, take, before);
+    int before, c = count_candidates(sh, tk, any, take, before);
     if (c == 0) return;
     if (tk.cnt + c > kSoft) {
         if (tk.cnt > k) compact(sh, tk, k);
@@ -194,18 +196,20 @@ __device__ __forceinline__ void add_candidates(Shared& sh, TopK& tk, int k, uint
         __syncthreads();                                      // sh.cut: the k-th largest, or 0 when fewer than k threads (quads) hold any
         // at least k keys are not below it: the bound for what follows, too
         tk.thr = sh.cut > tk.thr ? sh.cut : tk.thr;
-        chunk.keep(tk.thr, take);
-        c = count_candidates(sh, tk, take, before);
+        if (any) chunk.keep(tk.thr, take);
+        c = count_candidates(sh, tk, any, take, before);
     }
-    int at = tk.cnt + before;
+    if (any) {
+        int at = tk.cnt + before;
 #pragma unroll
-    for (int i = 0; i < EPT; i++) {
-        if (!take[i]) continue;
-        if ((take[i] >> lane) & 1) {
-            const int to = (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(take[i] >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)take[i], (uint32_t)at));
-            sh.score[to] = chunk.score(i); sh.col[to] = chunk.col(i);
+        for (int i = 0; i < EPT; i++) {
+            if (!take[i]) continue;
+            if ((take[i] >> lane) & 1) {
+                const int to = (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(take[i] >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)take[i], (uint32_t)at));
+                sh.score[to] = chunk.score(i); sh.col[to] = chunk.col(i);
+            }
+            at += __popcll(take[i]);
         }
-        at += __popcll(take[i]);
     }
     tk.cnt += c;
     tk.sorted = false;
@@ -348,8 +352,10 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(const T* __restrict_
             const float thr = tk.thr ? key_score(tk.thr) : -INFINITY;                         // later columns lose a tie: strictly greater
             uint64_t take[kEpt];
             const bool any = __ballot(top > thr) != 0;
+            if (any) {
 #pragma unroll
-            for (int i = 0; i < kEpt; i++) take[i] = any ? __ballot(v[i] > thr) : 0;           // false for NaN and for -inf
+                for (int i = 0; i < kEpt; i++) take[i] = __ballot(v[i] > thr);                 // false for NaN and for -inf
+            }
             struct Chunk {
                 const float (&v)[kEpt]; float top, thr; uint32_t base;
                 static constexpr int offset(int i) { return (i / V) * (kThreads * V) + i % V; }
@@ -365,10 +371,10 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(const T* __restrict_
                     const float x = cut ? key_score(cut) : -INFINITY;
                     const uint32_t c = key_col(cut);
 #pragma unroll
-                    for (int i = 0; i < kEpt; i++) take[i] = __ballot(v[i] > x) | (__ballot(v[i] == x) & __ballot(col(i) <= c) & take[i]);
+                    for (int i = 0; i < kEpt; i++) take[i] &= __ballot(v[i] > x) | (__ballot(v[i] == x) & __ballot(col(i) <= c));
                 }
             };
-            add_candidates(sh, tk, k, take, Chunk{v, top, thr, (uint32_t)base});
+            add_candidates(sh, tk, k, any, take, Chunk{v, top, thr, (uint32_t)base});
         }
     }
     if (k > 0 && !tk.sorted) compact(sh, tk, k);
@@ -424,7 +430,7 @@ __global__ __launch_bounds__(kThreads) void logprobs_join_kernel(const T* __rest
                 for (int i = 0; i < E; i++) take[i] &= __ballot(q[i] >= cut);
             }
         };
-        add_candidates(sh, tk, k, take, Keys{q});
+        add_candidates(sh, tk, k, true, take, Keys{q});
     }
     if (k > 0 && !tk.sorted) compact(sh, tk, k);
     const int cnt = tk.cnt;
