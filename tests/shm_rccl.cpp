@@ -38,7 +38,7 @@ struct Comm {
     char name[64] = {0};
     Header* hdr = nullptr; unsigned char* data = nullptr; size_t map_bytes = 0;
     long seq = 0;
-    void* stage = nullptr;                  // pinned staging for all-reduce results
+    void* stage = nullptr;                  // pinned staging of one collective's blocks
 };
 void spin_until(std::atomic<long>& a, long target) {
     const time_t t0 = time(nullptr);
@@ -63,8 +63,9 @@ int collective(Comm* c, const void* send, void* recv, size_t bytes, bool reduce,
     unsigned char* base = c->data + (size_t)slot * SLOT_BYTES;
     Header* h = c->hdr;
     spin_until(h->depart[slot], (long)c->world * use);                 // the slot's previous use has been read by every rank
-    if (hipMemcpyAsync(base + (size_t)c->rank * bytes, send, bytes, hipMemcpyDeviceToHost, s) != hipSuccess) return 1;
+    if (hipMemcpyAsync(c->stage, send, bytes, hipMemcpyDeviceToHost, s) != hipSuccess) return 1;
     if (hipStreamSynchronize(s) != hipSuccess) return 1;               // everything enqueued before the collective + the copy
+    memcpy(base + (size_t)c->rank * bytes, c->stage, bytes);
     h->arrive[slot].fetch_add(1, std::memory_order_acq_rel);
     spin_until(h->arrive[slot], (long)c->world * (use + 1));
     if (reduce) {
@@ -72,7 +73,10 @@ int collective(Comm* c, const void* send, void* recv, size_t bytes, bool reduce,
         else if (dtype == 7) reduce_into(static_cast<float*>(c->stage), base, bytes, count, c->world, op);
         else reduce_into(static_cast<int*>(c->stage), base, bytes, count, c->world, op);
         if (hipMemcpyAsync(recv, c->stage, bytes, hipMemcpyHostToDevice, s) != hipSuccess) return 1;
-    } else if (hipMemcpyAsync(recv, base, bytes * c->world, hipMemcpyHostToDevice, s) != hipSuccess) return 1;
+    } else {
+        memcpy(c->stage, base, bytes * c->world);
+        if (hipMemcpyAsync(recv, c->stage, bytes * c->world, hipMemcpyHostToDevice, s) != hipSuccess) return 1;
+    }
     if (hipStreamSynchronize(s) != hipSuccess) return 1;               // the slot (and the stage) may be reused after this
     h->depart[slot].fetch_add(1, std::memory_order_acq_rel);
     return 0;
@@ -114,8 +118,8 @@ __attribute__((visibility("default"))) int ncclCommInitRank(void** comm, int wor
     if (m == MAP_FAILED) { perror("[shm_rccl] mmap"); delete c; return 2; }
     c->hdr = static_cast<Header*>(m);                     // a fresh segment is zero-filled: every counter starts at 0
     c->data = static_cast<unsigned char*>(m) + 4096;
-    (void)hipHostRegister(m, c->map_bytes, hipHostRegisterDefault);       // async copies where the runtime can pin the mapping; pageable staging otherwise
-    if (hipHostMalloc(&c->stage, 1 << 20, hipHostMallocDefault) != hipSuccess) { delete c; return 1; }
+    // the mapping is not pinned in place: a runtime that refuses to pin memory which already exists reports that at the next HIP call
+    if (hipHostMalloc(&c->stage, SLOT_BYTES, hipHostMallocDefault) != hipSuccess) { delete c; return 1; }
     c->hdr->ready.fetch_add(1);
     const time_t t0 = time(nullptr);
     while (c->hdr->ready.load() < world) { usleep(100); if (time(nullptr) - t0 > 120) { fprintf(stderr, "[shm_rccl] rank %d: not all ranks attached\n", rank); return 2; } }
