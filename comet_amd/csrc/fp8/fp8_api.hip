@@ -56,6 +56,9 @@ void check_slots(const Fp8View& v, const int64_t* slots, int64_t first, int64_t 
     if (!slots) { check_range(v, first, n, "slots"); return; }
     if ((uintptr_t)slots % 8) COMET_FAIL(COMET_ERR_INVALID_ARG, "slots is not aligned to 8 bytes");
 }
+void check_scale(float scale) {      // scale * log2(e) has to be a float32 number
+    if (!(std::fabs(scale) > 0.0f) || !(std::fabs(scale) <= 0x1p126f)) COMET_FAIL(COMET_ERR_INVALID_ARG, "scale must be finite and not zero, and its magnitude at most 2^126");
+}
 void check_logprobs(int64_t m, int64_t n, int32_t k) {
     if (m < 0) COMET_FAIL(COMET_ERR_INVALID_ARG, "negative row count");
     if (n < 0 || n > ((int64_t)1 << 30)) COMET_FAIL(COMET_ERR_INVALID_ARG, "column count %lld outside [0, 2^30]", (long long)n);
@@ -154,7 +157,7 @@ int comet_logprobs_dev(comet_ctx* c, const void* scores, int dtype, int64_t ld, 
         if (!c) COMET_FAIL(COMET_ERR_INVALID_ARG, "context must not be null");
         check_logprobs(m, n, k);
         check_matrix(scores, dtype, ld, n == 0 ? 0 : m, n, "scores");
-        if (!(std::fabs(scale) > 0.0f) || !std::isfinite(scale)) COMET_FAIL(COMET_ERR_INVALID_ARG, "scale must be finite and not zero");
+        check_scale(scale);
         if (n_targets < 0) COMET_FAIL(COMET_ERR_INVALID_ARG, "negative target count");
         if (m > 0) {
             if (!logsum || !entropy) COMET_FAIL(COMET_ERR_INVALID_ARG, "out must not be null");
@@ -223,7 +226,7 @@ int comet_fp8_search(const comet_fp8_rows* r, int64_t first, int64_t n, const fl
         if (B < 0) COMET_FAIL(COMET_ERR_INVALID_ARG, "negative query count");
         check_logprobs(B, n, k);
         check_range(r->v, first, n, "rows");
-        if (!(std::fabs(scale) > 0.0f) || !std::isfinite(scale)) COMET_FAIL(COMET_ERR_INVALID_ARG, "scale must be finite and not zero");
+        check_scale(scale);
         if (B == 0) return (int)COMET_OK;
         if (!queries || (k > 0 && (!out_slots || !out_logprobs)) || !out_logsum || !out_entropy) COMET_FAIL(COMET_ERR_INVALID_ARG, "queries and out must not be null");
         HostCall g(r->c);

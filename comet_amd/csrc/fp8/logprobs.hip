@@ -449,7 +449,7 @@ int split_count(int64_t m, int64_t n) {
 
 template <bool NEG, class T> void logprobs_t(hipStream_t s, const LogProbsArgs& a) {
     const float scale = std::fabs(a.scale);
-    constexpr int64_t kPiece = (int64_t)1 << 24;
+    constexpr int64_t kPiece = (int64_t)1 << 22;        // (a launch has fewer than 2^32 threads)
     for (int64_t i = 0; i < a.m; i += kPiece) {
         const int64_t m = std::min(kPiece, a.m - i);
         const int splits = split_count(m, a.n);

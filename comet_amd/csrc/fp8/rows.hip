@@ -162,8 +162,9 @@ __global__ __launch_bounds__(256) void read_kernel(const uint8_t* __restrict__ c
 
 template <class T, int U> void write_t(hipStream_t s, const Fp8View& v, int32_t* last, const int64_t* slots, int64_t first, const T* x, int64_t ld, int64_t n) {
     const int rows = WriteShape<T, U>::rows(v.nb);
-    // rows are numbered with 32 bits in `last`; pieces follow each other on the stream, so the last row with a slot still stays
-    constexpr int64_t kPiece = (int64_t)1 << 30;
+    // a launch has fewer than 2^32 threads (and rows are numbered with 32 bits in `last`); pieces follow each other on the stream, so the last row with a
+    // slot still stays
+    constexpr int64_t kPiece = (int64_t)1 << 22;
     constexpr int64_t kScan = 64;           // up to this many rows a look through all slots is one load, and the marking launch is saved
     for (int64_t i = 0; i < n; i += kPiece) {
         const int m = (int)std::min(kPiece, n - i);
@@ -184,7 +185,7 @@ template <class T, int U> void write_t(hipStream_t s, const Fp8View& v, int32_t*
 
 template <class T> void read_t(hipStream_t s, const Fp8View& v, const int64_t* slots, int64_t first, T* out, int64_t ld, int64_t n) {
     constexpr int kRows = 256 / (kFp8Block / (16 / (int)sizeof(T)));
-    constexpr int64_t kPiece = (int64_t)1 << 30;
+    constexpr int64_t kPiece = (int64_t)1 << 24;        // (a launch has fewer than 2^32 threads)
     for (int64_t i = 0; i < n; i += kPiece) {
         const int64_t m = std::min(kPiece, n - i);
         hipLaunchKernelGGL((read_kernel<T>), dim3((unsigned)ceil_div(m, kRows)), dim3(256), 0, s, v.codes, v.scales, v.capacity, v.dim, v.nb, v.nb4,

@@ -378,7 +378,7 @@ COMET_API int comet_index_get_stat(const comet_index* idx, const char* name, dou
 /* ---- rows in 8-bit floating point --------------------------------------------------------------------
  * A store of `capacity` slots, each holding one row of `dim` numbers as e4m3 codes with a power-of-two scale per block of 128 consecutive
  * numbers (the last block padded with zeros): 1.01 bytes a number instead of 4, no training, any slot rewritten at any time. The reference's
- * nearest relative is its Int8Quantizer (quantizer.go; not used by any of its indexes); scores here are approximate where the indexes' are exact.
+ * nearest relatives are the quantisers of quantizer.go, which none of its indexes uses; scores here are of quantised rows where the indexes' are exact.
  *   A = largest finite |x| of the block; e = the least integer with A * 2^-e <= 448, at least -126 (a block of zeros: -126);
  *   code = e4m3(x * 2^-e), to nearest, ties to even (off by at most 2^-4 of the value, or 2^(e-10) where that is more); value = code * 2^e, exactly.
  * An infinite or NaN number is held as NaN; the others of its block keep their precision. (A float32 above 248 * 2^120 = 3.297e38 is held as 2^128, which
@@ -413,9 +413,10 @@ COMET_API int comet_fp8_scores_dev(const comet_fp8_rows* queries, int64_t q_firs
  * when counts_dev is NULL; entries behind them are not read),
  *   logsum = log sum_j exp(scale * s_j), entropy = -sum_j p_j log p_j (natural logarithms), logprobs (m x n_targets) = log p of the columns targets_dev[i][*],
  *   ids / top_logprobs (m x k) = the k columns of largest scale * s_j and their log p; equal scores: the lower column first. k <= 128.
- * scale may be negative (distances: the smallest are the best), not 0. An entry whose scaled score is -inf is masked: probability 0, never among the ids.
+ * scale may be negative (distances: the smallest are the best), not 0, |scale| <= 2^126. Two scores that differ by more than float32's largest number
+ * count as infinitely far apart. An entry of -inf (of +inf when scale is negative) is masked: probability 0, never among the ids.
  * Places no column is left for hold id -1 and log p -inf. A row with no unmasked entry: logsum -inf, entropy 0, log p -inf. A target outside [0, count):
- * -inf. A row with a NaN or a scaled score of +inf among its entries: logsum, entropy and log p NaN; a NaN is never among the ids.
+ * -inf. A row with a NaN or the other infinity among its entries: logsum, entropy and log p NaN; a NaN is never among the ids.
  * n <= 2^30. `work_dev`: comet_logprobs_work_bytes(m, n, k) bytes (0 for short rows), 16-byte aligned, written and read by the call; the size for
  * (m, n, k) is enough for every smaller m, n, k. Two calls that may run at once need two. */
 COMET_API int comet_logprobs_work_bytes(int64_t m, int64_t n, int32_t k, size_t* out_bytes);

@@ -201,6 +201,30 @@ def test_scores_of_whole_numbers_are_exact(ctx, dev, m, n, dim):
     Q.close(); R.close()
 
 
+@pytest.mark.parametrize("m,n,dim", [(4, 30001, 300), (5, 100003, 100), (20, 80001, 200), (130, 70001, 130), (300, 40003, 100), (520, 33000, 300), (256, 66000, 20)])
+def test_scores_over_many_tiles(ctx, dev, m, n, dim):
+    """more tiles than run at once, of one block and of a few: a workgroup's next tile arrives while it finishes the last"""
+    rng = np.random.default_rng(n)
+    q, r = rng.integers(-7, 8, (m, dim)).astype(np.float32), rng.integers(-7, 8, (n, dim)).astype(np.float32)
+    Q, R = Fp8Rows(ctx, m, dim), Fp8Rows(ctx, n, dim)
+    write(dev, Q, q); write(dev, R, r)
+    assert same(scores(dev, Q, m, R, n), q.astype(np.float64) @ r.astype(np.float64).T)
+    assert same(scores(dev, Q, m, R, n - 5, "bf16", pad=3, first=2), ref.from_bf16_bits(ref.to_bf16_bits(q @ r[2:n - 3].T)))
+    Q.close(); R.close()
+
+
+def test_a_pair_has_one_score(ctx, dev):
+    """the score of a query and a row does not depend on what they are multiplied with: few queries, tiles of every shape, any window"""
+    n, dim, m = 9000, 700, 600
+    q, r = rows_of(31, m, dim), rows_of(32, n, dim)
+    Q, R = Fp8Rows(ctx, m, dim), Fp8Rows(ctx, n, dim)
+    write(dev, Q, q); write(dev, R, r)
+    whole = scores(dev, Q, m, R, n)
+    for q0, mm, r0, nn in ((0, 1, 0, n), (17, 3, 5, 777), (100, 5, 11, 4001), (33, 64, 1, 300), (1, 599, 8000, 1000), (300, 129, 257, 8000)):
+        assert same(scores(dev, Q, mm, R, nn, q_first=q0, first=r0), whole[q0:q0 + mm, r0:r0 + nn])
+    Q.close(); R.close()
+
+
 @pytest.mark.parametrize("m", [1, 40, 300])
 def test_scores_of_non_finite_and_far_apart_rows(ctx, dev, m):
     """a NaN stays in its row's and its query's scores; blocks at both ends of the scales' range keep their products"""
@@ -448,12 +472,12 @@ def test_refusals(ctx, dev):
     o = dev.new((64,), np.float32)
     big = LogProbs(ctx, 4, 20000, 10)
     ok = dict(out_logsum=o, out_entropy=o, k=0)
-    small = LogProbs(ctx, 4, 100, 10)
+    small, wide = LogProbs(ctx, 4, 100, 10), dev.new((40000,), np.float32)
     for f in (lambda: LogProbs(ctx, 1, 10, 129), lambda: LogProbs(ctx, 1, 2 ** 30 + 1, 1), lambda: LogProbs(ctx, -1, 1, 1), lambda: big.run_dev(x, "f32", 1, 10, scale=0.0, **ok),
-              lambda: big.run_dev(x, "f32", 1, 10, scale=float("inf"), **ok), lambda: big.run_dev(x, "f32", 2, 10, ld=9, **ok), lambda: big.run_dev(0, "f32", 2, 10, **ok),
+              lambda: big.run_dev(x, "f32", 1, 10, scale=float("inf"), **ok), lambda: big.run_dev(x, "f32", 1, 10, scale=1e38, **ok), lambda: big.run_dev(x, "f32", 2, 10, ld=9, **ok), lambda: big.run_dev(0, "f32", 2, 10, **ok),
               lambda: big.run_dev(x, "f32", 1, 10, out_logsum=0, out_entropy=o), lambda: big.run_dev(x, "f32", 1, 10, n_targets=1, **ok),
               lambda: big.run_dev(x, "f32", 1, 10, out_logsum=o, out_entropy=o, k=1), lambda: big.run_dev(x, "f32", 1, 10, n_targets=-1, **ok),
-              lambda: small.run_dev(x, "f32", 1, 9000, **ok), lambda: big.run_dev(x, "f32", 1, 10, out_logsum=o, out_entropy=o, k=-1)):
+              lambda: small.run_dev(wide, "f32", 1, 40000, **ok), lambda: big.run_dev(x, "f32", 1, 10, out_logsum=o, out_entropy=o, k=-1)):
         with pytest.raises(CometError):
             f()
     for p in (R, S, big, small):
