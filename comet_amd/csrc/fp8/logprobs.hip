@@ -62,7 +62,8 @@ template <int X> __device__ __forceinline__ uint64_t xor_lane64(uint64_t v) { re
 // of 64 and 128 go through sh.best (256 keys are 33 lane steps and 3 of LDS; counting each key's rank instead was 64-bit compares of all with all, 8 us a
 // time with four workgroups on a CU).
 template <int N> __device__ void sort_keys(Shared& sh, uint64_t (&key)[N]) {
-    const int t = threadIdx.x;
+    int t = threadIdx.x;
+    asm volatile("" : "+v"(t));        // the network's lane masks are made here: kept across the chunks they crowd the scalar registers out
     auto keep = [&](uint64_t& mine, uint64_t other, bool lower, bool down) { mine = ((mine > other) == (lower == down)) ? mine : other; };
     auto lanes = [&](auto X, int size) {
         constexpr int x = decltype(X)::value;
@@ -94,7 +95,8 @@ template <int N> __device__ void sort_keys(Shared& sh, uint64_t (&key)[N]) {
 
 // the same for 64 keys in one wave
 __device__ __forceinline__ uint64_t sort_wave(uint64_t key) {
-    const int t = threadIdx.x & 63;
+    int t = threadIdx.x & 63;
+    asm volatile("" : "+v"(t));
     auto step = [&](auto X, int size) {
         constexpr int x = decltype(X)::value;
         const uint64_t other = xor_lane64<x>(key);
@@ -132,19 +134,17 @@ __device__ void compact(Shared& sh, TopK& tk, int k) {
         sort_keys<2>(sh, key);
         if (t < k) sh.put(t, key[0]);                       // k <= 128 < 256 < cnt
         __syncthreads();
-    } else {                                                // rows whose best columns crowd into few threads
-        int p = 1024;
-        while (p < cnt) p <<= 1;                            // positions from cnt on are never stored and hold the smallest key
-        for (int size = 2; size <= p; size <<= 1) {
-            for (int stride = size >> 1; stride > 0; stride >>= 1) {
-                for (int h = t; h < p / 2; h += kThreads) {
-                    // every merge descending: its first step compares mirrored positions
-                    const int i = 2 * h - (h & (stride - 1));
-                    const int j = stride == (size >> 1) ? (i & ~(size - 1)) + size - 1 - (i & (size - 1)) : i + stride;
-                    if (j < cnt) { const uint64_t x = sh.key(i), y = sh.key(j); if (x < y) { sh.put(i, y); sh.put(j, x); } }
-                }
-                __syncthreads();
+    } else {                                                // rows whose best columns crowd into few threads: the k best of the first 512, then of those and the next
+        for (int from = 0, held = 0; from < cnt; from += 2 * kThreads - held, held = k) {
+            uint64_t key[2];
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                const int p = i * kThreads + t, at = p < held ? p : from + p - held;
+                key[i] = at < cnt ? sh.key(at) : 0;
             }
+            sort_keys<2>(sh, key);
+            if (t < k) sh.put(t, key[0]);                   // the round's keys lie behind the first k or are in registers
+            __syncthreads();
         }
     }
     tk.cnt = cnt < k ? cnt : k;
@@ -189,11 +189,14 @@ __device__ __forceinline__ void add_candidates(Shared& sh, TopK& tk, int k, bool
                 const uint64_t key = sort_wave(sh.best[threadIdx.x]);
                 if ((int)threadIdx.x == k - 1) sh.cut = key;
             }
-        } else {
+            __syncthreads();
+        }
+        if (k > kThreads / 8 || sh.cut == 0) {                // the few columns of a row's end crowd into fewer than k quads
             sort_keys<1>(sh, best);
             if ((int)threadIdx.x == k - 1) sh.cut = best[0];
+            __syncthreads();
         }
-        __syncthreads();                                      // sh.cut: the k-th largest, or 0 when fewer than k threads (quads) hold any
+        // sh.cut: the k-th largest, or 0 when fewer than k threads hold any
         // at least k keys are not below it: the bound for what follows, too
         tk.thr = sh.cut > tk.thr ? sh.cut : tk.thr;
         if (any) chunk.keep(tk.thr, take);
@@ -279,7 +282,7 @@ __device__ __forceinline__ void finish_row(const Shared& sh, const Stats& st, in
     }
 }
 
-// Workgroup (row, split): columns [split * span, ...) of the row's count in chunks of 8192, each thread 32 of them in 16-byte pieces.
+// Workgroup (row, split): columns [split * span, ...) of the row's count in chunks of 4096, each thread 16 of them in 16-byte pieces.
 template <bool NEG, class T>
 __global__ __launch_bounds__(kThreads) void logprobs_kernel(const T* __restrict__ scores, int64_t ld, int n, const int32_t* __restrict__ counts, float scale,
                                                             const int32_t* __restrict__ targets, int n_targets, int k, int splits, float* __restrict__ logprobs,

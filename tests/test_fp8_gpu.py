@@ -349,6 +349,17 @@ def test_logprobs_of_rows_in_awkward_orders(ctx, dev, m, n, k, scale, kind):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("k", [1, 20, 32, 33, 100, 128])
+def test_logprobs_of_rows_that_end_early_in_a_chunk(ctx, dev, dtype, k):
+    """rows whose last columns are more candidates than are held at once and lie in few threads"""
+    counts = np.array([513, 514, 600, 640, 641, 800, 1023, 1025, 2000, 4096 + 513, 4096 + 600, 8192 + 639, 0, 512], np.int32)
+    n = int(counts.max())
+    for kind in ("normal", "ascending", "ties"):
+        s = ref.decode(ref.encode(score_rows(n + k, len(counts), n, kind), dtype), dtype)
+        check_logprobs(run_logprobs(ctx, dev, s, dtype, n, 1, counts, 2.0, None, k), s, n, counts, 2.0, None, k)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("scale", [1.0, -3.0])
 @pytest.mark.parametrize("n", [200, 20000])
 def test_logprobs_of_masked_ragged_and_non_finite_rows(ctx, dev, dtype, scale, n):
