@@ -18,6 +18,9 @@ constexpr int kThreads = 256, kWaves = kThreads / 64, kEpt = 16, kChunk = kThrea
 // Candidate buffer: the k best so far and one chunk's survivors. When more than kSoft would be held, the chunk is cut to the keys not below the k-th
 // largest of the 256 threads' largest keys: only the k threads above that bound hold survivors, kEpt each. (Up to k = 32 quads of threads do.)
 constexpr int kSoft = 512, kCap = kLogProbsMaxK + kEpt * kLogProbsMaxK;
+// Splits of a row: enough workgroups for four per CU. A row of up to four chunks is not split: a second launch costs more than the chunks one after the other
+// (1 x 10000, k = 10: 10.6 us a pass, against 14.5 split in three).
+constexpr int64_t kGroups = 1024, kWhole = 4;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 struct Stats { float m, s, w; int bad; };   // maximum, S, W in units of log2 (w = sum e * t, t = d * log2 e); bad: a NaN among masked entries only (any other is in s)
@@ -171,12 +174,12 @@ template <int EPT> __device__ __forceinline__ int count_candidates(Shared& sh, T
 }
 
 // Adds this chunk's candidates: take[i] holds the lanes whose element i is one (uniform across the wave). Of `chunk`: best() is the thread's largest key (0:
-// none), keep(cut, take) drops what lies below cut, score(i) and col(i) are an element.
+// none), keep(cut, take) drops what lies below cut, score(i) and col(i) are an element. Returns whether the workgroup had any.
 template <int EPT, class Chunk>
-__device__ __forceinline__ void add_candidates(Shared& sh, TopK& tk, int k, bool any, uint64_t (&take)[EPT], const Chunk& chunk) {
+__device__ __forceinline__ bool add_candidates(Shared& sh, TopK& tk, int k, bool any, uint64_t (&take)[EPT], const Chunk& chunk) {
     const int lane = threadIdx.x & 63;
     int before, c = count_candidates(sh, tk, any, take, before);
-    if (c == 0) return;
+    if (c == 0) return false;
     if (tk.cnt + c > kSoft) {
         if (tk.cnt > k) compact(sh, tk, k);
         uint64_t best[1] = {chunk.best()};
@@ -217,6 +220,7 @@ __device__ __forceinline__ void add_candidates(Shared& sh, TopK& tk, int k, bool
     tk.cnt += c;
     tk.sorted = false;
     if (tk.cnt >= k + kThreads) compact(sh, tk, k);
+    return true;
 }
 
 template <int X = 1, class F> __device__ __forceinline__ float reduce_wave(float v, F join) {      // over the 64 lanes, always in the same order
@@ -387,11 +391,12 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(const T* __restrict_
         finish_row<NEG>(sh, st, row, x, count, cnt, row_targets, target, n_targets, k, scale, logprobs, logsum, entropy, ids, top_logprobs);
     } else {
         if (threadIdx.x == 0) part_stats[blockIdx.x] = st;
-        for (int i = threadIdx.x; i < k; i += kThreads) part_keys[(int64_t)blockIdx.x * k + i] = i < cnt ? sh.key(i) : 0;
+        for (int i = threadIdx.x; i < k; i += kThreads) part_keys[(row * k + i) * splits + split] = i < cnt ? sh.key(i) : 0;
     }
 }
 
-// joins a row's splits
+// Joins a row's splits. Their keys lie rank by rank: the best of all splits first, then the second best, ... A turn sees every split at least once, so when it has
+// no key above the bound no later one has (1 x 1000000, k = 100: 245 splits, 24500 keys, of which two or three turns read 2048 each).
 template <bool NEG, class T>
 __global__ __launch_bounds__(kThreads) void logprobs_join_kernel(const T* __restrict__ scores, int64_t ld, int n, const int32_t* __restrict__ counts, float scale,
                                                                  const int32_t* __restrict__ targets, int n_targets, int k, int splits, float* __restrict__ logprobs,
@@ -399,6 +404,7 @@ __global__ __launch_bounds__(kThreads) void logprobs_join_kernel(const T* __rest
                                                                  const Stats* __restrict__ part_stats, const uint64_t* __restrict__ part_keys) {
     __shared__ Shared sh;
     constexpr int E = 8;
+    static_assert(kThreads * E >= kGroups);
     const int64_t row = blockIdx.x;
     int count = n;
     if (counts) { count = counts[row]; count = count < 0 ? 0 : (count > n ? n : count); }
@@ -433,7 +439,7 @@ __global__ __launch_bounds__(kThreads) void logprobs_join_kernel(const T* __rest
                 for (int i = 0; i < E; i++) take[i] &= __ballot(q[i] >= cut);
             }
         };
-        add_candidates(sh, tk, k, true, take, Keys{q});
+        if (!add_candidates(sh, tk, k, true, take, Keys{q})) break;
     }
     if (k > 0 && !tk.sorted) compact(sh, tk, k);
     const int cnt = tk.cnt;
@@ -441,9 +447,6 @@ __global__ __launch_bounds__(kThreads) void logprobs_join_kernel(const T* __rest
     finish_row<NEG>(sh, st, row, x, count, cnt, row_targets, target, n_targets, k, scale, logprobs, logsum, entropy, ids, top_logprobs);
 }
 
-// Splits of a row: enough workgroups for four per CU. A row of up to four chunks is not split: a second launch costs more than the chunks one after the other
-// (1 x 10000, k = 10: 10.6 us a pass, against 14.5 split in three).
-constexpr int64_t kGroups = 1024, kWhole = 4;
 int64_t chunk_count(int64_t n) { return std::max<int64_t>(1, ceil_div(n, kChunk)); }
 int split_count(int64_t m, int64_t n) {
     const int64_t chunks = chunk_count(n);
