@@ -29,6 +29,13 @@ def _dtype(name: str) -> int:
     return _DTYPE[name]
 
 
+def _i32(x: int, what: str) -> int:
+    x = int(x)
+    if not -(1 << 31) <= x < 1 << 31:
+        raise ValueError(f"{what} {x} does not fit 32 bits")
+    return x
+
+
 def _host(a: np.ndarray):
     return a.ctypes.data_as(C.c_void_p)
 
@@ -48,7 +55,7 @@ class Fp8Rows:
     def __init__(self, ctx: Context, capacity: int, dim: int):
         self.ctx, self.lib = ctx, ctx.lib
         h = C.c_void_p()
-        check(self.lib.comet_fp8_create(ctx.h, int(capacity), int(dim), C.byref(h)))
+        check(self.lib.comet_fp8_create(ctx.h, int(capacity), _i32(dim, "dimension"), C.byref(h)))
         self.h = h
         self.capacity, self.dim = int(capacity), int(dim)
 
@@ -115,9 +122,10 @@ class Fp8Rows:
         if q.ndim != 2 or q.shape[1] != self.dim:
             raise ValueError(f"query dimension mismatch: expected {self.dim}, got {q.shape[-1]}")
         n = self.capacity - first if n is None else n
-        B, kk = q.shape[0], max(int(k), 0)
+        B, k = _i32(q.shape[0], "query count"), _i32(k, "k")
+        kk = k if 0 <= k <= 128 else 0           # any other is refused below
         r = Fp8SearchResult(np.empty((B, kk), np.int64), np.empty((B, kk), np.float32), np.empty(B, np.float32), np.empty(B, np.float32))
-        check(self.lib.comet_fp8_search(self.h, int(first), int(n), _host(q), B, C.c_float(scale), int(k), _host(r.slots), _host(r.logprobs), _host(r.logsum), _host(r.entropy)))
+        check(self.lib.comet_fp8_search(self.h, int(first), int(n), _host(q), B, C.c_float(scale), k, _host(r.slots), _host(r.logprobs), _host(r.logsum), _host(r.entropy)))
         return r
 
 
@@ -128,7 +136,7 @@ class LogProbs:
     def __init__(self, ctx: Context, m: int, n: int, k: int):
         self.ctx, self.lib = ctx, ctx.lib
         size = C.c_size_t()
-        check(self.lib.comet_logprobs_work_bytes(int(m), int(n), int(k), C.byref(size)))
+        check(self.lib.comet_logprobs_work_bytes(int(m), int(n), _i32(k, "k"), C.byref(size)))
         self.work_bytes = size.value
         self.work = ctx.alloc(self.work_bytes) if self.work_bytes else 0
 
@@ -149,5 +157,5 @@ class LogProbs:
         """scores: m x n, ``ld`` elements apart; counts (m), targets (m x n_targets) and out_ids (m x k) are int32, the other outputs float32"""
         p = lambda a: C.c_void_p(a or None)  # noqa: E731
         check(self.lib.comet_logprobs_dev(self.ctx.h, p(scores), _dtype(dtype), int(n if ld is None else ld), int(m), int(n), p(counts), C.c_float(scale), p(targets),
-                                          int(n_targets), int(k), p(out_logprobs), p(out_logsum), p(out_entropy), p(out_ids), p(out_top_logprobs), p(self.work),
+                                          _i32(n_targets, "target count"), _i32(k, "k"), p(out_logprobs), p(out_logsum), p(out_entropy), p(out_ids), p(out_top_logprobs), p(self.work),
                                           self.work_bytes, C.c_void_p(self.ctx.stream if stream is None else int(stream))))

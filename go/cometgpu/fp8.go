@@ -38,6 +38,9 @@ type Fp8Result struct {
 
 // NewFp8Rows allocates the store; every slot holds zeros.
 func NewFp8Rows(ctx *Context, capacity int64, dim int) (*Fp8Rows, error) {
+	if dim <= 0 || dim > 1<<20 {
+		return nil, fmt.Errorf("dimension must be positive and at most 2^20")
+	}
 	r := &Fp8Rows{ctx: ctx, capacity: capacity, dim: dim}
 	if rc := C.comet_fp8_create(ctx.h, C.int64_t(capacity), C.int32_t(dim), &r.h); rc != C.COMET_OK {
 		return nil, lastError(rc)
@@ -107,8 +110,8 @@ func (r *Fp8Rows) Search(queries [][]float32, first, n int64, k int, scale float
 	if B == 0 {
 		return nil, nil
 	}
-	if k < 0 {
-		return nil, fmt.Errorf("k must not be negative")
+	if k < 0 || k > 128 {
+		return nil, fmt.Errorf("k %d outside [0, 128]", k)
 	}
 	flat, err := r.flatten(queries)
 	if err != nil {

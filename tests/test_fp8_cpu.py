@@ -26,6 +26,20 @@ def test_null_handles_are_refused():
         assert lib.comet_logprobs_work_bytes(m, n, k, C.byref(z)) == _lib.ERR_INVALID_ARG, (m, n, k)
 
 
+def test_numbers_beyond_32_bits_are_refused_before_they_are_cut():
+    from types import SimpleNamespace
+
+    from comet_amd import Fp8Rows, LogProbs
+    ctx = SimpleNamespace(lib=_lib.load(), h=None, stream=0)
+    for f in (lambda: Fp8Rows(ctx, 8, (1 << 32) + 8), lambda: LogProbs(ctx, 1, 10, (1 << 32) + 1)):
+        with pytest.raises(ValueError, match="32 bits"):
+            f()
+    p = LogProbs(ctx, 1, 10, 1)
+    for kw in (dict(k=1 << 32), dict(n_targets=(1 << 32) + 1)):
+        with pytest.raises(ValueError, match="32 bits"):
+            p.run_dev(16, "f32", 1, 10, out_logsum=16, out_entropy=16, **kw)
+
+
 def test_workspace_of_a_large_call_serves_smaller_ones():
     lib = _lib.load()
 
