@@ -7,7 +7,12 @@
 //
 // The best k columns ride on the same pass: a workgroup keeps the candidates that exceed its k-th best so far in LDS and sorts them when they get many.
 // A key is (score, column) in 64 bits, larger is better, equal scores to the lower column; keys are unique, so the result does not depend on the order in
-// which candidates arrive. Candidates wait as the score's own bits over the column's complement and become keys when they are sorted. Bound by reading the scores once.
+// which candidates arrive. Candidates wait as the score's own bits over the column's complement and become keys when they are sorted.
+//
+// Bound by reading the scores once where rows are long: 256 x 1000000 float32 take 175 us (5.9 TB/s) without the best columns and 195 us (5.3 TB/s) with the best
+// 100; 1000 ragged rows of up to 30011 bfloat16 take 16 and, with the best 20, 26 us (a call that reads nothing takes 8): a row is eight chunks, and a chunk with
+// candidates costs its workgroup a barrier and the candidates' stores. Chunks of 16 numbers a thread: 32 took 223 us for the first, 8 177 us for 1024 x 200000
+// bfloat16 that now take 154.
 #include "fp8.hpp"
 #include "lanes.hpp"
 

@@ -2,7 +2,9 @@
 //
 // A block is 128 consecutive values of a row. With A the largest finite |x| of the block, e is the least integer with A * 2^-e <= 448 (the largest
 // e4m3 number) and the codes are e4m3(x * 2^-e), rounded to nearest even: multiplying by a power of two is exact, so a code is off by half a step of
-// e4m3 and by nothing else (2^-4 of the value; 2^-10 * 2^e below 2^-6 * 2^e). Both directions move each byte once and are bound by HBM.
+// e4m3 and by nothing else (2^-4 of the value; 2^-10 * 2^e below 2^-6 * 2^e). Both directions move each byte once and are
+// bound by HBM: 131072 x 768 float32 are written in 120 us (4.2 TB/s; the marking launch before it 6.5 us) and read as bfloat16 in 53 us (5.7 TB/s), 25600 x 768
+// scattered rows are read as float32 in 19 us (5.1 TB/s).
 #include "fp8.hpp"
 #include "lanes.hpp"
 
@@ -203,7 +205,7 @@ void launch_fp8_write(hipStream_t s, const Fp8View& v, int32_t* last, const int6
         else if (dtype == COMET_F16) write_t<_Float16, U>(s, v, last, slots, first, (const _Float16*)x, ld, n);
         else write_t<__bf16, U>(s, v, last, slots, first, (const __bf16*)x, ld, n);
     };
-    // blocks a group: two read a bulk of rows at the rate of a copy (131072 x 768 float32 and back: 176 us, against 219 with one and 189 with four); rows of one
+    // blocks a group: two read a bulk of rows at the rate of a copy (131072 x 768 float32 and back as bfloat16: 175 us, against 219 with one and 189 with four); rows of one
     // and of three blocks leave no group half empty
     if (v.nb == 1) blocks(std::integral_constant<int, 1>{});
     else if (v.nb == 3) blocks(std::integral_constant<int, 3>{});

@@ -13,6 +13,12 @@
 //
 // The order of k inside a block is free as long as both operands use the same one (a block has one scale), so lane l takes row l % 16 and the 16-byte
 // pieces l / 16 and 4 + l / 16 of its 128: every load instruction covers 64 consecutive bytes of 16 rows.
+//
+// What bounds it: one query reads the rows at 5.6 TB/s (1 x 1M x 768: 139 us). 256 x 1M x 768 in float32 (410 us) moves 1.8 GB at 4.4 TB/s, more than half of it
+// written. 2047 x 30011 x 2000 (208 us, 1.18 PFLOP/s) is bound by instruction issue: 1.9 vector instructions, 1.5 of them conversions, go with each matrix
+// instruction, and the matrix units are busy for 64% of the time a CU has work. Reading operands one step ahead with a single barrier a block (227 us), an order
+// with every conversion between matrix instructions (equal, and registers spill for 16-bit scores) and converting once a workgroup into bfloat16 LDS tiles
+// (239 us: twice the LDS traffic) were measured and left out; so were tiles of 128 x 128 a wave (the accumulators leave no registers).
 #include "fp8.hpp"
 
 namespace comet {
@@ -52,7 +58,7 @@ template <class T> __device__ __forceinline__ void store4(T* row, int64_t j, int
 }
 
 // Up to four queries: the stored rows stream once through the registers, each wave 64 rows against an operand of queries whose blocks come out of the caches
-// (1 x 1M x 768: 142 us, 5.5 TB/s, against 149 with the smallest tile below; 16 queries: 184 against 175).
+// (1 x 1M x 768: 139 us, 5.6 TB/s, against 149 with the smallest tile below; 16 queries: 184 against 175).
 constexpr int kStreamQueries = 4;
 template <class T>
 __global__ __launch_bounds__(256) void scores_stream_kernel(const uint8_t* __restrict__ qc, const uint8_t* __restrict__ qs, int m, const uint8_t* __restrict__ rc,
