@@ -15,7 +15,9 @@
 // RWMutex discipline (searches share the read lock; Add / Train / Flush / ReadFrom take the write lock), BM25
 // tokenisation (uax29 words + NFKC + lower-casing, bm25_index.go:154-166). All distance arithmetic, list scans,
 // graph traversal, BM25 accumulation and top-k selection run on the GPU and return the reference's results bit for bit
-// (see tests/ in the backend repository: every path is compared with a CPU restatement of the Go loops).
+// (see tests/ in the backend repository: every path of the indexes is compared with a CPU restatement of the Go loops).
+//
+// Fp8Rows (fp8.go) is not one of comet's interfaces: a store of rows in 8-bit floating point whose scores are those of the quantised rows.
 //
 // Place this directory at github.com/wizenheimer/comet/cometgpu (it imports the parent package) and point cgo at the
 // backend checkout: CGO_CFLAGS=-I<backend>/include CGO_LDFLAGS="-L<backend>/comet_amd -lcomet_hip".
