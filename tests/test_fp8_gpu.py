@@ -348,6 +348,15 @@ def test_logprobs_of_rows_in_awkward_orders(ctx, dev, m, n, k, scale, kind):
     check_logprobs(run_logprobs(ctx, dev, s, "f32", n, 0, None, scale, None, k), s, n, None, scale, None, k)
 
 
+@pytest.mark.parametrize("kind", ["normal", "ties", "ascending", "descending", "equal"])
+@pytest.mark.parametrize("m,k", [(1, 128), (2, 1), (3, 30)])
+def test_logprobs_of_rows_in_hundreds_of_splits(ctx, dev, m, k, kind):
+    """the best columns of all splits, or of one split alone, are found however few turns the joining takes"""
+    n = 1000003
+    s = score_rows(m + k, m, n, kind)
+    check_logprobs(run_logprobs(ctx, dev, s, "f32", n, 0, None, 1.5, None, k), s, n, None, 1.5, None, k)
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("k", [1, 20, 32, 33, 100, 128])
 def test_logprobs_of_rows_that_end_early_in_a_chunk(ctx, dev, dtype, k):
