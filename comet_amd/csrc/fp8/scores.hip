@@ -15,10 +15,12 @@
 // pieces l / 16 and 4 + l / 16 of its 128: every load instruction covers 64 consecutive bytes of 16 rows.
 //
 // What bounds it: one query reads the rows at 5.6 TB/s (1 x 1M x 768: 139 us). 256 x 1M x 768 in float32 (410 us) moves 1.8 GB at 4.4 TB/s, more than half of it
-// written. 2047 x 30011 x 2000 (208 us, 1.18 PFLOP/s) is bound by instruction issue: 1.9 vector instructions, 1.5 of them conversions, go with each matrix
-// instruction, and the matrix units are busy for 64% of the time a CU has work. Reading operands one step ahead with a single barrier a block (227 us), an order
-// with every conversion between matrix instructions (equal, and registers spill for 16-bit scores) and converting once a workgroup into bfloat16 LDS tiles
-// (239 us: twice the LDS traffic) were measured and left out; so were tiles of 128 x 128 a wave (the accumulators leave no registers).
+// written. Long rows run at the rate of the card's matrix units under load: 2048 x 32768 x 4096 at 1.36 PFLOP/s, as fast as a library product of bfloat16 rows
+// (8192^3: 1.37 - 1.40); leaving the conversions out changes nothing there (429 us against 425), never filling a buffer again 366. 2047 x 30011 x 2000 (208 us,
+// 1.18 PFLOP/s) adds what a tile costs besides its products, about 5 us a round of the chip in which all tiles are stored at once, and 944 tiles in 3.7 rounds.
+// Measured and left out: the next block's fill in front of a tile's stores, behind a barrier of its own (430 us for 256 x 1M x 768, against 413), operands read
+// one step ahead with a single barrier late in a block (441), a fixed order with a conversion or two between matrix instructions (421, and registers spill for
+// 16-bit scores), conversion once a workgroup into bfloat16 LDS tiles (459), workgroups started apart so that their stores do not meet (408 - 418).
 #include "fp8.hpp"
 
 namespace comet {
