@@ -123,10 +123,10 @@ template <int QT, int WQ, int WAVES> struct TileShape {
 __device__ __forceinline__ void fill16(const uint8_t* base /* uniform */, uint32_t offset, uint32_t lds /* uniform */) {
     const uint64_t b = (uint64_t)base;
     const uint64_t sb = ((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(b >> 32)) << 32) | (uint32_t)__builtin_amdgcn_readfirstlane((int)b);
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %0, %1" :: "v"(offset), "s"(sb), "s"(__builtin_amdgcn_readfirstlane((int)lds)) : "memory", "m0");
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %0, %1" :: "v"(offset), "s"(sb), "s"(__builtin_amdgcn_readfirstlane((int)lds)) : "memory");
 }
 __device__ __forceinline__ void fill4(const uint8_t* address, uint32_t lds /* uniform */) {
-    asm volatile("s_mov_b32 m0, %1\n\ts_nop 3\n\tglobal_load_lds_dword %0, off" :: "v"(address), "s"(__builtin_amdgcn_readfirstlane((int)lds)) : "memory", "m0");
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 3\n\tglobal_load_lds_dword %0, off" :: "v"(address), "s"(__builtin_amdgcn_readfirstlane((int)lds)) : "memory");
 }
 __device__ __forceinline__ uint32_t lds_address(const void* p) { return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)p; }
 template <int N> __device__ __forceinline__ void wait_vm() { asm volatile("s_waitcnt vmcnt(%0)" :: "n"(N) : "memory"); }
