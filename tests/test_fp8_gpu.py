@@ -3,7 +3,7 @@
 Tolerances. Quantised values, rows read back and ids are compared exactly. A score is a sum of K exact products formed in float32: each of the K additions
 is off by at most one step (2^-23) of a partial sum that never exceeds sum |q r|, so by K * 2^-23 * sum |q r| in all, plus half a step of the output type.
 A log-probability is d - log S with d = (s - max) * scale: two roundings of d and one of the difference (2^-23 (|d| + |lp|)), and log S, whose S is off
-relatively by the additions a thread makes one after the other (32 per chunk of 8192 columns, 2^-24 each, and eight joins), by the exponent's rounding
+relatively by the additions a thread makes one after the other (16 per chunk of 4096 columns, 2^-24 each, and eight joins), by the exponent's rounding
 (3 * 2^-24 |t| weighted by p: the mean of |d| is at most H + log S) and by the exponential's last place: together 2^-23 (16 n / 8192 + 16 + |d| + |lp| + 3 (H + log S)).
 The entropy adds log S and a mean of |d| with the same relative error; logsum the rounding of max * scale."""
 import threading
@@ -464,6 +464,55 @@ def test_searches_from_several_threads(ctx):
     [i.start() for i in t]; [i.join() for i in t]
     assert not bad
     R.close()
+
+
+# ---- calls of more than one launch ---------------------------------------------------------------------------------
+def test_writes_and_reads_of_more_rows_than_one_launch_takes(ctx, dev):
+    n, capacity = (1 << 22) + 70, 1000
+    rng = np.random.default_rng(5)
+    x, slots = rng.standard_normal((n, 1)).astype(np.float32), rng.integers(-1, capacity, n)
+    slots[5], slots[(1 << 22) + 3] = 7, 7                     # one slot in both launches
+    R = Fp8Rows(ctx, capacity, 1)
+    write(dev, R, x, slots=slots)
+    last = np.full(capacity + 1, -1)
+    last[slots] = np.arange(n)                                # numpy keeps the last of equal indices
+    want = ref.held(x[last[:capacity]])
+    assert same(R.read(np.arange(capacity)), want)
+    n = (1 << 24) + 300
+    slots = rng.integers(-1, capacity + 1, n)
+    got = read(dev, R, n, "f16", slots=slots)[:, 0]
+    want = np.append(want[:, 0].astype(np.float16).astype(np.float64), [0.0, 0.0])
+    assert (got == want[np.where((slots < 0) | (slots >= capacity), capacity, slots)]).all()
+    R.close()
+
+
+def test_scores_of_more_queries_and_rows_than_one_launch_takes(ctx, dev):
+    rng = np.random.default_rng(6)
+    q, r = rng.integers(-7, 8, ((1 << 16) + 9, 3)).astype(np.float32), rng.integers(-7, 8, (6, 3)).astype(np.float32)
+    Q, R = Fp8Rows(ctx, len(q), 3), Fp8Rows(ctx, 6, 3)
+    write(dev, Q, q); write(dev, R, r)
+    assert same(scores(dev, Q, len(q), R, 6, pad=1), q.astype(np.float64) @ r.astype(np.float64).T)
+    Q.close(); R.close()
+    n, m = (1 << 24) + 40, 5
+    q, r = rng.integers(-7, 8, (m, 1)).astype(np.float32), rng.integers(-7, 8, (n, 1)).astype(np.float32)
+    Q, R = Fp8Rows(ctx, m, 1), Fp8Rows(ctx, n, 1)
+    write(dev, Q, q); write(dev, R, r)
+    for mm in (3, m):                                         # both kernels
+        out = dev.new((mm, n), np.float32)
+        R.scores_dev(Q, mm, out)
+        got = dev.get(out, (mm, n), np.float32)
+        for a, b in ((0, 500), ((1 << 24) - 300, n)):
+            assert (got[:, a:b] == q[:mm] * r[a:b, 0]).all()
+    Q.close(); R.close()
+
+
+def test_logprobs_of_more_rows_than_one_launch_takes(ctx, dev):
+    m, n = (1 << 22) + 9, 3
+    s = score_rows(9, m, n)
+    counts = np.random.default_rng(1).integers(0, n + 1, m).astype(np.int32)
+    got = run_logprobs(ctx, dev, s, "f32", n, 0, counts, -2.0, None, 1)
+    for a, b in ((0, 300), ((1 << 22) - 100, m)):
+        check_logprobs({x: v[a:b] for x, v in got.items()}, s[a:b], n, counts[a:b], -2.0, None, 1)
 
 
 # ---- refusals ----------------------------------------------------------------------------------------------------------
