@@ -21,7 +21,7 @@ inline size_t dtype_size(int dtype) { return dtype == COMET_F32 ? 4 : 2; }
 // Every launch below goes to the given stream, allocates nothing, waits for nothing and is capturable.
 
 // rows x[i] (n x dim, `ld` elements apart) -> slot slots[i], or first + i when slots == nullptr; slots outside [0, capacity) are skipped; of rows
-// with the same slot the last one stays. `last`: one int32 per slot, -1 between calls.
+// with the same slot the last one stays. `last`: one int32 per slot, -1 between calls. The codes behind a row's dim must be 0 already.
 void launch_fp8_write(hipStream_t s, const Fp8View& v, int32_t* last, const int64_t* slots, int64_t first, const void* x, int dtype, int64_t ld, int64_t n);
 // out[i] (n x dim, `ld` elements apart) <- the values slot slots[i] (or first + i) holds; slots outside [0, capacity) give zeros
 void launch_fp8_read(hipStream_t s, const Fp8View& v, const int64_t* slots, int64_t first, void* out, int dtype, int64_t ld, int64_t n);

@@ -239,6 +239,7 @@ int comet_fp8_search(const comet_fp8_rows* r, int64_t first, int64_t n, const fl
         q.capacity = piece;
         float* x = c->salloc<float>((size_t)piece * dim);
         q.codes = c->salloc<uint8_t>((size_t)piece * q.nb * kFp8Block); q.scales = c->salloc<uint8_t>((size_t)piece * q.nb4);
+        if (dim % kFp8Block) HIP_CHECK(hipMemsetAsync(q.codes, 0, (size_t)piece * q.nb * kFp8Block, c->stream));       // a store's padding is zero before its first write
         float* scores = c->salloc<float>((size_t)piece * std::max<int64_t>(1, n));
         void* work = c->scratch_alloc(work_bytes + 16);
         float *ls = c->salloc<float>(piece), *en = c->salloc<float>(piece), *tl = c->salloc<float>((size_t)piece * k + 1);

@@ -130,6 +130,33 @@ def test_values_where_the_format_can_go_wrong(ctx, dev):
     store.close()
 
 
+@pytest.mark.parametrize("dtype,pad,offset", [("f32", 0, 0), ("f32", 3, 1), ("f16", 1, 0), ("bf16", 0, 0), ("bf16", 5, 3)])
+@pytest.mark.parametrize("dim", [1, 7, 16, 17, 32, 33, 40, 63, 64, 65, 100, 128])
+def test_rows_of_up_to_one_block(ctx, dev, dtype, pad, offset, dim):
+    """narrow rows share a wave: consecutive slots, few rows and many rows to given slots, some named twice, some outside"""
+    rng = np.random.default_rng(dim)
+    capacity = 700
+    R = Fp8Rows(ctx, capacity, dim)
+    held = np.zeros((capacity, dim))
+    for n, given in ((333, False), (50, True), (600, True)):
+        x = ref.decode(ref.encode((rng.standard_normal((n, dim)) * np.exp(4 * rng.standard_normal((n, 1)))).astype(np.float32), dtype), dtype)
+        slots = rng.integers(-2, capacity + 2, n) if given else np.arange(100, 100 + n)
+        write(dev, R, x, dtype, pad, slots if given else None, 0 if given else 100, offset)
+        h = ref.held(x)
+        for i, at in enumerate(slots):
+            if 0 <= at < capacity:
+                held[at] = h[i]
+        want = ref.decode(ref.encode(held.astype(np.float32), dtype), dtype)
+        assert same(read(dev, R, capacity, dtype, pad, None, 0, offset), want)
+        assert same(read(dev, R, n, dtype, pad, slots, 0, offset), np.where(((slots >= 0) & (slots < capacity))[:, None], want[np.clip(slots, 0, capacity - 1)], 0.0))
+    one = np.ones((3, dim), np.float32)                     # what lies behind the rows' width adds nothing to a product
+    Q = Fp8Rows(ctx, 3, dim)
+    write(dev, Q, one)
+    got, want, mag = scores(dev, Q, 3, R, capacity), held.sum(axis=1), np.abs(held).sum(axis=1)
+    assert ((np.abs(got - want) <= dim * 2.0 ** -23 * mag) | (np.isnan(got) & np.isnan(want))).all()       # float16 rows hold infinities: NaN
+    Q.close(); R.close()
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("n", [2, 64, 65, 1000, 5000])
 def test_slots_repeated_and_outside(ctx, dev, n, dtype):
@@ -434,6 +461,26 @@ def test_write_score_rank_and_read_back_as_one_run(ctx, dev, B, n, dim, k, scale
     assert same(H.read(np.arange(cap)), read(dev, R, cap))
     for o in (R, Q, H):
         o.close()
+
+
+def test_search_of_narrow_rows_behind_one_of_wide_rows(ctx):
+    """the queries' padding is zero whatever an earlier call left in the workspace"""
+    wide = Fp8Rows(ctx, 300, 128)
+    wide.write(rows_of(60, 300, 128), np.arange(300))
+    narrow = Fp8Rows(ctx, 500, 20)
+    x, q = rows_of(61, 500, 20), rows_of(62, 9, 20)
+    narrow.write(x, np.arange(500))
+    hq, hx = ref.held(q), ref.held(x)
+    s = hq @ hx.T
+    for turn in range(3):
+        wide.search(np.full((200, 128), 3.0, np.float32), 10, 1.0)
+        r = narrow.search(q, 1, 50.0)
+        best = s.argmax(axis=1)
+        assert (r.slots[:, 0] == best).all()
+        want = (50 * (s - s.max(axis=1, keepdims=True)))
+        # 20 additions of products below 1 move a score by 20 * 2^-23 at most, times the scale
+        assert (np.abs(r.logprobs[:, 0] + np.log(np.exp(want).sum(axis=1))) <= 50 * 2 * 20 * 2.0 ** -23 + 64 * 2.0 ** -23).all()
+    wide.close(); narrow.close()
 
 
 def test_search_of_many_queries_runs_in_pieces(ctx):
