@@ -119,14 +119,15 @@ template <int QT, int WQ, int WAVES> struct TileShape {
 };
 
 // The fills are asm statements: around the compiler's own form of them every LDS read that follows would wait for the fill just issued (it cannot tell the
-// buffers apart). The waits are written out where a buffer changes hands. No register outputs; M0 holds the LDS address of the wave's part.
+// buffers apart). The waits are written out where a buffer changes hands. No register outputs. The LDS address of the wave's part is an operand in M0, so
+// the compiler knows what M0 holds; the s_nop are the five wait states between a vector instruction that wrote a scalar register and a load that takes it.
 __device__ __forceinline__ void fill16(const uint8_t* base /* uniform */, uint32_t offset, uint32_t lds /* uniform */) {
     const uint64_t b = (uint64_t)base;
     const uint64_t sb = ((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(b >> 32)) << 32) | (uint32_t)__builtin_amdgcn_readfirstlane((int)b);
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %0, %1" :: "v"(offset), "s"(sb), "s"(__builtin_amdgcn_readfirstlane((int)lds)) : "memory");
+    asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %0, %1" :: "v"(offset), "s"(sb), "{m0}"(__builtin_amdgcn_readfirstlane((int)lds)) : "memory");
 }
 __device__ __forceinline__ void fill4(const uint8_t* address, uint32_t lds /* uniform */) {
-    asm volatile("s_mov_b32 m0, %1\n\ts_nop 3\n\tglobal_load_lds_dword %0, off" :: "v"(address), "s"(__builtin_amdgcn_readfirstlane((int)lds)) : "memory");
+    asm volatile("s_nop 4\n\tglobal_load_lds_dword %0, off" :: "v"(address), "{m0}"(__builtin_amdgcn_readfirstlane((int)lds)) : "memory");
 }
 __device__ __forceinline__ uint32_t lds_address(const void* p) { return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)p; }
 template <int N> __device__ __forceinline__ void wait_vm() { asm volatile("s_waitcnt vmcnt(%0)" :: "n"(N) : "memory"); }

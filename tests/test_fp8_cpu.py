@@ -1,5 +1,7 @@
 """What the 8-bit row store's entry points refuse before they touch a device, and the plain restatements the GPU tests compare with."""
 import ctypes as C
+import re
+from pathlib import Path
 
 import numpy as np
 import pytest
@@ -77,3 +79,16 @@ def test_reference_bf16_round_trip():
     f = ref.from_bf16_bits(u)
     ok = ~np.isnan(f)
     assert (ref.to_bf16_bits(f)[ok] == u[ok]).all()
+
+
+def test_asm_names_the_registers_it_takes():
+    """a load into LDS takes its address from M0: an operand of the asm statement, never written behind the compiler's back"""
+    seen = 0
+    for f in sorted((Path(__file__).resolve().parent.parent / "comet_amd" / "csrc" / "fp8").glob("*.h*")):
+        for stmt in re.findall(r"asm volatile\((.*?)\);", f.read_text(), re.S):
+            code, _, operands = stmt.partition("::")
+            assert not re.search(r"\bm0\b", code), (f.name, stmt)
+            if "_lds_" in code:
+                assert '"{m0}"' in operands, (f.name, stmt)
+                seen += 1
+    assert seen
