@@ -43,6 +43,7 @@ template <class F> inline int guarded(F&& f) {
     try { return f(); }
     catch (const StatusError& s) { return s.code; }
     catch (const HipError& h) {
+        (void)hipGetLastError();        // reported here: the next call's launch check must not take it for its own
         return set_error(COMET_ERR_HIP, "HIP error %d (%s) in %s at %s:%d", (int)h.e, hipGetErrorString(h.e), h.what, h.file, h.line);
     }
     catch (const std::bad_alloc&) { return set_error(COMET_ERR_HIP, "host allocation failed"); }
