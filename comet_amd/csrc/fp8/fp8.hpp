@@ -2,6 +2,9 @@
 // A stored row is `nb` blocks of 128 e4m3 codes (row-major, the last block padded with zero codes) and one power-of-two scale byte
 // (e8m0: 2^(byte - 127)) per block, `nb4` = nb rounded up to 4 bytes apart per row, so that four blocks' scales are one dword.
 #pragma once
+#include <tuple>
+#include <utility>
+
 #include "../index.hpp"
 
 namespace comet {
@@ -17,6 +20,16 @@ struct Fp8View {            // device memory of one store
 };
 
 inline size_t dtype_size(int dtype) { return dtype == COMET_F32 ? 4 : 2; }
+
+// Launches a kernel and checks what the launch itself returned: an error that another call left in the runtime neither stops a write half way (marked slots
+// whose rows never arrive would lose every later row) nor is taken from that call.
+template <class... P, class... A> void launch_kernel(void (*kernel)(P...), int64_t groups, int threads, size_t lds, hipStream_t s, A... args) {
+    std::tuple<P...> held(static_cast<P>(args)...);
+    std::apply([&](auto&... a) {
+        void* list[] = {(void*)&a...};
+        HIP_CHECK(hipLaunchKernel((const void*)kernel, dim3((unsigned)groups), dim3((unsigned)threads), list, lds, s));
+    }, held);
+}
 
 // Every launch below goes to the given stream, allocates nothing, waits for nothing and is capturable.
 

@@ -472,14 +472,9 @@ template <bool NEG, class T> void logprobs_t(hipStream_t s, const LogProbsArgs& 
         float* lp = a.n_targets ? a.logprobs + i * a.n_targets : nullptr;
         int32_t* ids = a.k ? a.ids + i * a.k : nullptr;
         float* tl = a.k ? a.top_logprobs + i * a.k : nullptr;
-        hipLaunchKernelGGL((logprobs_kernel<NEG, T>), dim3((unsigned)(m * splits)), dim3(kThreads), 0, s, x, a.ld, a.n, counts, scale, targets, a.n_targets, a.k, splits,
-                           lp, a.logsum + i, a.entropy + i, ids, tl, ps, pk);
-        LAUNCH_CHECK();
-        if (splits > 1) {
-            hipLaunchKernelGGL((logprobs_join_kernel<NEG, T>), dim3((unsigned)m), dim3(kThreads), 0, s, x, a.ld, a.n, counts, scale, targets, a.n_targets, a.k, splits,
-                               lp, a.logsum + i, a.entropy + i, ids, tl, ps, pk);
-            LAUNCH_CHECK();
-        }
+        launch_kernel(logprobs_kernel<NEG, T>, m * splits, kThreads, 0, s, x, a.ld, a.n, counts, scale, targets, a.n_targets, a.k, splits, lp, a.logsum + i, a.entropy + i, ids, tl, ps, pk);
+        if (splits > 1)
+            launch_kernel(logprobs_join_kernel<NEG, T>, m, kThreads, 0, s, x, a.ld, a.n, counts, scale, targets, a.n_targets, a.k, splits, lp, a.logsum + i, a.entropy + i, ids, tl, ps, pk);
     }
 }
 }  // namespace

@@ -237,26 +237,23 @@ template <class Launch> void write_pieces(hipStream_t s, const Fp8View& v, int32
         } else if (m <= kScan) {
             launch(std::integral_constant<int, 1>{}, i, m, slots + i, (int64_t)0);
         } else {
-            hipLaunchKernelGGL(mark_kernel, dim3((unsigned)ceil_div(m, 256)), dim3(256), 0, s, slots + i, m, v.capacity, last);
-            LAUNCH_CHECK();
+            launch_kernel(mark_kernel, ceil_div(m, 256), 256, 0, s, slots + i, m, v.capacity, last);
             launch(std::integral_constant<int, 2>{}, i, m, slots + i, (int64_t)0);
         }
-        LAUNCH_CHECK();
     }
 }
 
 template <class T, int U> void write_t(hipStream_t s, const Fp8View& v, int32_t* last, const int64_t* slots, int64_t first, const T* x, int64_t ld, int64_t n) {
     const int rows = WriteShape<T, U>::rows(v.nb);
     write_pieces(s, v, last, slots, first, n, [&](auto dup, int64_t i, int m, const int64_t* slots_i, int64_t first_i) {
-        hipLaunchKernelGGL((write_kernel<T, U, decltype(dup)::value>), dim3((unsigned)ceil_div(m, rows)), dim3(256), 0, s, x + i * ld, ld, m, v.dim, slots_i, first_i, v.codes, v.scales,
-                           v.capacity, v.nb, v.nb4, last, rows);
+        launch_kernel(write_kernel<T, U, decltype(dup)::value>, ceil_div(m, rows), 256, 0, s, x + i * ld, ld, m, v.dim, slots_i, first_i, v.codes, v.scales, v.capacity, v.nb, v.nb4, last,
+                      rows);
     });
 }
 template <class T, int L> void write_short_t(hipStream_t s, const Fp8View& v, int32_t* last, const int64_t* slots, int64_t first, const T* x, int64_t ld, int64_t n) {
     constexpr int rows = 256 / L * (L > 8 ? L / 8 : 1);
     write_pieces(s, v, last, slots, first, n, [&](auto dup, int64_t i, int m, const int64_t* slots_i, int64_t first_i) {
-        hipLaunchKernelGGL((write_short_kernel<T, L, decltype(dup)::value>), dim3((unsigned)ceil_div(m, rows)), dim3(256), 0, s, x + i * ld, ld, m, v.dim, slots_i, first_i, v.codes,
-                           v.scales, v.capacity, last);
+        launch_kernel(write_short_kernel<T, L, decltype(dup)::value>, ceil_div(m, rows), 256, 0, s, x + i * ld, ld, m, v.dim, slots_i, first_i, v.codes, v.scales, v.capacity, last);
     });
 }
 
@@ -269,11 +266,9 @@ template <class T> void read_t(hipStream_t s, const Fp8View& v, const int64_t* s
         const int64_t m = std::min(kPiece, n - i);
         const int64_t* slots_i = slots ? slots + i : nullptr;
         if (v.dim <= kFp8Block / 2)
-            hipLaunchKernelGGL((read_short_kernel<T>), dim3((unsigned)ceil_div(m << shift, 256)), dim3(256), 0, s, v.codes, v.scales, v.capacity, v.dim, slots_i, first + i, out + i * ld, ld, m,
-                               shift);
+            launch_kernel(read_short_kernel<T>, ceil_div(m << shift, 256), 256, 0, s, v.codes, v.scales, v.capacity, v.dim, slots_i, first + i, out + i * ld, ld, m, shift);
         else
-            hipLaunchKernelGGL((read_kernel<T>), dim3((unsigned)ceil_div(m, kRows)), dim3(256), 0, s, v.codes, v.scales, v.capacity, v.dim, v.nb, v.nb4, slots_i, first + i, out + i * ld, ld, m);
-        LAUNCH_CHECK();
+            launch_kernel(read_kernel<T>, ceil_div(m, kRows), 256, 0, s, v.codes, v.scales, v.capacity, v.dim, v.nb, v.nb4, slots_i, first + i, out + i * ld, ld, m);
     }
 }
 }  // namespace

@@ -267,7 +267,7 @@ void launch_tiles(hipStream_t s, const uint8_t* qc, const uint8_t* qs, int m, co
     HIP_CHECK(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
     const int mt = (int)ceil_div(m, Shape::BM), nt = (int)ceil_div(n, Shape::BN);
     const int64_t groups = std::min<int64_t>(256 * per_cu, round_up((int64_t)mt * nt, 8));
-    hipLaunchKernelGGL(kernel, dim3((unsigned)groups), dim3(WAVES * 64), bytes, s, qc, qs, m, rc, rs, n, nb, nb4, out, ld, mt, nt);
+    launch_kernel(kernel, groups, WAVES * 64, bytes, s, qc, qs, m, rc, rs, n, nb, nb4, out, ld, mt, nt);
 }
 
 // Which tile: the fewest rounds of the chip (256 tiles of 256 x 256, 512 of the smaller ones, two a CU), each weighted with its measured time: a round of the
@@ -288,13 +288,12 @@ template <class T> void scores_t(hipStream_t s, const Fp8View& q, int64_t q_firs
         const uint8_t *qc = q.codes + (q_first + i) * q.row_bytes(), *qs = q.scales + (q_first + i) * q.nb4;
         const uint8_t *rc = r.codes + (first + j) * r.row_bytes(), *rs = r.scales + (first + j) * r.nb4;
         T* o = out + i * ld + j;
-        if (mi <= kStreamQueries) hipLaunchKernelGGL((scores_stream_kernel<T>), dim3((unsigned)ceil_div(nj, 256)), dim3(256), 0, s, qc, qs, mi, rc, rs, nj, r.nb, r.nb4, o, ld);
+        if (mi <= kStreamQueries) launch_kernel(scores_stream_kernel<T>, ceil_div(nj, 256), 256, 0, s, qc, qs, mi, rc, rs, nj, r.nb, r.nb4, o, ld);
         else switch (pick_tile(mi, nj)) {
             case Tile::large: launch_tiles<T, 8, 2, 8, 2>(s, qc, qs, mi, rc, rs, nj, r.nb, r.nb4, o, ld); break;
             case Tile::middle: launch_tiles<T, 4, 2, 4, 2>(s, qc, qs, mi, rc, rs, nj, r.nb, r.nb4, o, ld); break;
             case Tile::small: launch_tiles<T, 2, 2, 4, 2>(s, qc, qs, mi, rc, rs, nj, r.nb, r.nb4, o, ld); break;
         }
-        LAUNCH_CHECK();
     }
 }
 }  // namespace

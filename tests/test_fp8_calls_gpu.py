@@ -26,3 +26,17 @@ def test_a_store_that_does_not_fit_leaves_no_error_behind(ctx, dev):
         write(dev, R, x, slots=np.arange(100))
         assert same(read(dev, R, 100), ref.held(x))
     R.close()
+
+
+def test_an_error_of_another_call_does_not_stop_these(ctx, dev):
+    """an error left in the runtime by the caller's own HIP call: the row store's calls check their own launches, and a write to slots arrives whole, as do later ones"""
+    n, dim = 300, 200
+    x, y = rows_of(2, n, dim), rows_of(3, n, dim)
+    R = Fp8Rows(ctx, n, dim)
+    assert ctx.lib.hipSetDevice(10 ** 6) != 0         # refused: the process has no such device
+    write(dev, R, x[::-1], slots=np.arange(n)[::-1])
+    assert same(read(dev, R, n), ref.held(x))
+    write(dev, R, y[:70], slots=np.arange(70))        # rows of lower numbers than the first call's in the same slots
+    assert same(read(dev, R, n), ref.held(np.concatenate([y[:70], x[70:]])))
+    ctx.lib.hipGetLastError()
+    R.close()
