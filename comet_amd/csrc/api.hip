@@ -28,7 +28,7 @@ struct CallGuard {   // serialise calls on a context, bind the device, reset the
     // other than 0 starts behind whatever non-search work lane 0 was last given (Ctx::lane0_fence): the queries may still be being written there
     CallGuard(Ctx* c_, int lane) : c(c_), lk(c_->mu), search(true) {
         c->check_indexes("entry of an asynchronous search"); c->bind();
-        if (!c->async_seen) { c->switch_lane(0); c->fence_lane0(); c->async_seen = true; }      // the first one: everything lane 0 holds so far is what it must start behind
+        c->begin_async();
         c->switch_lane(lane); c->scratch_reset(); c->follow_lane0();
     }
     ~CallGuard() {
@@ -84,6 +84,7 @@ int comet_ctx_create(int device_id, comet_ctx** out) {
         const int pr_a = normal ? std::min(pr_least, pr_greatest + 1) : pr_greatest;          // numerically lower = more urgent
         const int pr_b = std::min(pr_least, pr_a + 1);
         HIP_CHECK(hipStreamCreateWithPriority(&c->stream, hipStreamNonBlocking, pr_a));
+        c->lane0 = c->stream;
         for (int l = 1; l < Ctx::kMaxLanes; l++) HIP_CHECK(hipStreamCreateWithPriority(&c->parked[l].stream, hipStreamNonBlocking, l < 4 ? pr_a : pr_b));
         *out = c;
         return COMET_OK;
@@ -114,7 +115,7 @@ int comet_ctx_destroy(comet_ctx* c) {
     });
 }
 int comet_ctx_sync(comet_ctx* c) { return guarded([&] { std::lock_guard<std::recursive_mutex> lk(c->mu); c->bind(); c->sync(); return COMET_OK; }); }
-void* comet_ctx_stream(comet_ctx* c) { std::lock_guard<std::recursive_mutex> lk(c->mu); return (void*)(c->cur_lane == 0 ? c->stream : c->parked[0].stream); }
+void* comet_ctx_stream(comet_ctx* c) { return (void*)c->lane0; }
 int comet_ctx_fence(comet_ctx* c) { return guarded([&] { std::lock_guard<std::recursive_mutex> lk(c->mu); c->bind(); c->switch_lane(0); c->fence_lane0(); return COMET_OK; }); }
 int comet_dev_alloc(comet_ctx* c, size_t bytes, void** out) { return guarded([&] { c->bind(); HIP_CHECK(hipMalloc(out, bytes ? bytes : 4)); return COMET_OK; }); }
 int comet_dev_free(comet_ctx* c, void* p) { return guarded([&] { c->bind(); if (p) HIP_CHECK(hipFree(p)); return COMET_OK; }); }

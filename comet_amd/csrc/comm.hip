@@ -199,7 +199,7 @@ int comet_index_search_sharded_async(comet_index* idx, comet_comm* cm, const flo
         struct LaneBack { Ctx* c; ~LaneBack() { if (c->cur_lane != 0) { c->mark_dirty(); c->switch_lane(0); } } } lane_back{c};
         // the first asynchronous search of the context (same sequence as api.hip's CallGuard(c, lane)): everything lane 0 holds so far — the queries'
         // upload or generation — is what a search on lanes 1.. must start behind; from here on non-search calls keep the fence current
-        if (!c->async_seen) { c->switch_lane(0); c->fence_lane0(); c->async_seen = true; }
+        c->begin_async();
         { const int m = std::min(c->lanes, idx->max_lanes()); c->switch_lane(m > 1 ? (idx->lane_toggle = (idx->lane_toggle + 1) % m) : 0); }
         c->scratch_reset();
         c->follow_lane0();          // lanes 1..: behind the non-search work lane 0 was last given (the queries' upload / generation)

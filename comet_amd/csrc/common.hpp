@@ -80,6 +80,7 @@ struct ProfEntry { double ms = 0; int64_t n = 0; };
 struct Ctx {
     int device = 0;
     hipStream_t stream = nullptr;
+    hipStream_t lane0 = nullptr;  // lane 0's stream, whichever lane is current: set once, read without the lock
     hipDeviceProp_t prop{};
     std::recursive_mutex mu;  // serialises calls that share the scratch arena / stream
     // scratch arena: bump allocator over one device allocation, reset at the start of every call.
@@ -116,16 +117,33 @@ struct Ctx {
     // (CallGuard) or when the caller asks for it after enqueueing its own kernels on comet_ctx_stream() (comet_ctx_fence); a search on
     // another lane waits for the newest record. Searches on lane 0 do NOT move the fence: a search on lane 1 must not queue up behind the
     // search that lane 0 is running (that would serialise the lanes).
+    // Calls that only queue (comet_fp8_*_dev, comet_logprobs_dev) do not take `mu`, which a blocking call holds for as long as it runs: the fence has a mutex of
+    // its own, held for one record or one wait. A call queues its work first and looks at `async_seen` under that mutex afterwards, so either the first
+    // asynchronous search has not recorded the fence yet, or the call records it.
+    std::mutex fence_mu;
     hipEvent_t lane0_fence = nullptr; bool lane0_fence_set = false;
     bool async_seen = false;        // an asynchronous search has been issued on this context: only then do non-search calls record the fence (a context that is only
                                     // ever used through the blocking calls re-recorded the event after every call for nobody — thousands of records on one event)
     hipEvent_t fork_ev = nullptr;   // segments_search: the other lanes start behind what lane 0 holds at the call (owned by the context: an event belongs to a device)
-    void fence_lane0() {            // lane 0 current
+    void record_fence() {           // fence_mu held
         if (!lane0_fence) HIP_CHECK(hipEventCreateWithFlags(&lane0_fence, hipEventDisableTiming));
-        HIP_CHECK(hipEventRecord(lane0_fence, stream));
+        HIP_CHECK(hipEventRecord(lane0_fence, lane0));
         lane0_fence_set = true;
     }
+    void fence_lane0() { std::lock_guard<std::mutex> lk(fence_mu); record_fence(); }
+    void begin_async() {            // an asynchronous search is about to be queued. The first one: everything lane 0 holds so far is what it must start behind
+        std::lock_guard<std::mutex> lk(fence_mu);
+        if (!async_seen) { record_fence(); async_seen = true; }
+    }
+    void queued_on_lane0() {        // by a call that does not hold `mu`. A stream under capture takes no event of the context's
+        std::lock_guard<std::mutex> lk(fence_mu);
+        if (!async_seen) return;
+        hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+        HIP_CHECK(hipStreamIsCapturing(lane0, &st));
+        if (st == hipStreamCaptureStatusNone) record_fence();
+    }
     void follow_lane0() {           // the current lane (>= 1) starts behind the newest fence of lane 0
+        std::lock_guard<std::mutex> lk(fence_mu);
         if (cur_lane != 0 && lane0_fence_set) HIP_CHECK(hipStreamWaitEvent(stream, lane0_fence, 0));
     }
     void quiesce_alt() {         // called with lane 0 current: the other lanes idle

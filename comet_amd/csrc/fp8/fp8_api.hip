@@ -26,16 +26,8 @@ struct HostCall {
 };
 
 // Work queued on lane 0's own stream is what later asynchronous searches start behind (as for every other call that queues there). Other streams are the
-// caller's to order, and a stream under capture takes no event of the context's.
-void queued(Ctx* c, hipStream_t s) {
-    std::lock_guard<std::recursive_mutex> lk(c->mu);
-    if (!c->async_seen || s != (c->cur_lane == 0 ? c->stream : c->parked[0].stream)) return;
-    hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
-    HIP_CHECK(hipStreamIsCapturing(s, &st));
-    if (st != hipStreamCaptureStatusNone) return;
-    c->switch_lane(0);
-    c->fence_lane0();
-}
+// caller's to order. Neither takes the context's mutex: a call on device arrays does not stand behind another thread's search or upload.
+void queued(Ctx* c, hipStream_t s) { if (s == c->lane0) c->queued_on_lane0(); }
 
 void check_dtype(int dtype) { if (dtype != COMET_F32 && dtype != COMET_F16 && dtype != COMET_BF16) COMET_FAIL(COMET_ERR_INVALID_ARG, "unknown element type %d", dtype); }
 void check_rows(const comet_fp8_rows* r) { if (!r) COMET_FAIL(COMET_ERR_INVALID_ARG, "rows must not be null"); }
