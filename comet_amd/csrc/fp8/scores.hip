@@ -107,14 +107,13 @@ __global__ __launch_bounds__(256) void scores_stream_kernel(const uint8_t* __res
     for (int i = 0; i < 4; i++) if (i < m) store4(out + i * ld, n0 + lane * 4, n, v4f{acc[0][i], acc[1][i], acc[2][i], acc[3][i]});
 }
 
-// More queries: a workgroup of WAVES waves walks tiles of BM queries x BN rows, block by block, through a ring of STAGES LDS buffers that the memory pipe
-// fills STAGES - 1 blocks ahead, across tiles: the next tile's first blocks arrive while this one is finished and stored. A wave multiplies QT * 16 queries
-// with 64 rows. One buffer holds the codes of a block (queries, then rows: 128 bytes each) and the rows' and queries' dword of scales. 16-byte piece c
-// of code row r lies at place c ^ (r & 7), so that the sixteen rows of an operand read fall on all banks (the fill permutes its global addresses, not its
-// LDS ones).
+// More queries: a workgroup of WAVES waves walks tiles of BM queries x BN rows, block by block, through two LDS buffers that the memory pipe fills one block
+// ahead, across tiles: the next tile's first block arrives while this one is finished and stored. A wave multiplies QT * 16 queries with 64 rows. One buffer
+// holds the codes of a block (queries, then rows: 128 bytes each) and the rows' and queries' dword of scales. 16-byte piece c of code row r lies at place
+// c ^ (r & 7), so that the sixteen rows of an operand read fall on all banks (the fill permutes its global addresses, not its LDS ones).
 template <int QT, int WQ, int WAVES> struct TileShape {
     static constexpr int BM = WQ * QT * 16, BN = WAVES / WQ * 64, rows = BM + BN, codes = rows * kFp8Block, stage = codes + WAVES * 256;
-    static constexpr int FQ = BM / (8 * WAVES), FR = BN / (8 * WAVES), fills = FQ + FR + 1;      // fill instructions a wave issues per block: 8 code rows each, and one for scales
+    static constexpr int FQ = BM / (8 * WAVES), FR = BN / (8 * WAVES);      // fill instructions a wave issues per block: 8 code rows each (and one for scales)
     static_assert(BM % (8 * WAVES) == 0 && BN % (8 * WAVES) == 0 && rows <= WAVES * 64, "the waves share the fills evenly");
 };
 
@@ -132,12 +131,12 @@ __device__ __forceinline__ void fill4(const uint8_t* address, uint32_t lds /* un
 __device__ __forceinline__ uint32_t lds_address(const void* p) { return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)p; }
 template <int N> __device__ __forceinline__ void wait_vm() { asm volatile("s_waitcnt vmcnt(%0)" :: "n"(N) : "memory"); }
 
-template <class T, int QT, int WQ, int WAVES, int STAGES>
+template <class T, int QT, int WQ, int WAVES>
 __global__ __launch_bounds__(WAVES * 64, 2) void scores_tile_kernel(const uint8_t* __restrict__ qc, const uint8_t* __restrict__ qs, int m, const uint8_t* __restrict__ rc,
                                                                       const uint8_t* __restrict__ rs, int n, int nb, int nb4, T* __restrict__ out, int64_t ld, int m_tiles, int n_tiles) {
     using Shape = TileShape<QT, WQ, WAVES>;
     extern __shared__ __align__(16) uint8_t lds[];
-    constexpr int RT = 4, BM = Shape::BM, BN = Shape::BN, FQ = Shape::FQ, FR = Shape::FR, F = Shape::fills, ST = QT * 4;
+    constexpr int RT = 4, BM = Shape::BM, BN = Shape::BN, FQ = Shape::FQ, FR = Shape::FR;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wq = (wave % WQ) * QT * 16, wr = (wave / WQ) * RT * 16;
     const int64_t row_bytes = (int64_t)nb * kFp8Block;
@@ -173,12 +172,11 @@ __global__ __launch_bounds__(WAVES * 64, 2) void scores_tile_kernel(const uint8_
 #pragma unroll
         for (int i = 0; i < FR; i++) fill16(fr_base + f_b * kFp8Block, fr[i], to + BM * kFp8Block + (i * WAVES + wave) * 1024);
         fill4(f_scale + (f_b & ~3), to + Shape::codes + wave * 256);
-        f_stage = f_stage + 1 == STAGES ? 0 : f_stage + 1;
+        f_stage ^= 1;
         if (++f_b == nb) { f_b = 0; f_tile += groups; if (f_tile < t_end) fill_tile(); }
     };
     fill_tile();
-#pragma unroll
-    for (int i = 0; i < STAGES - 1; i++) if (i < steps) fill();
+    fill();
 
     v4f acc[RT][QT];
 #pragma unroll
@@ -186,13 +184,13 @@ __global__ __launch_bounds__(WAVES * 64, 2) void scores_tile_kernel(const uint8_
 #pragma unroll
         for (int v = 0; v < QT; v++) acc[t][v] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
     int tile = t0, b = 0, stage = 0;
-    int stored = STAGES;            // steps since the last full tile was stored
+    bool stored = false;            // the step before stored a tile that lay inside the matrix: QT * 4 store instructions a wave
     for (int step = 0; step < steps; step++) {
-        // Block `step` has arrived when only what was issued behind its fill is left: the fills of the STAGES - 2 blocks after it and one tile's stores (ST per
-        // wave when the tile lay inside the matrix), if they came since. At the end, where fewer fills follow, everything is waited for.
-        if (step + STAGES - 2 >= steps) wait_vm<0>();
-        else if (stored < STAGES - 1) wait_vm<(STAGES - 2) * F + ST>();
-        else wait_vm<(STAGES - 2) * F>();
+        // Block `step` has arrived when nothing is left that was issued before its fill or in it: behind it came only such a tile's stores, and a tile at the
+        // edge, whose number of stores differs from wave to wave, is waited for with them.
+        if (stored) wait_vm<QT * 4>();
+        else wait_vm<0>();
+        stored = false;
         __builtin_amdgcn_s_barrier();       // ... for every wave, and every wave is done with the buffer that is filled next
         asm volatile("" ::: "memory");
         const uint8_t* buf = lds + stage * Shape::stage;
@@ -209,7 +207,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void scores_tile_kernel(const uint8_
             for (int t = 0; t < RT; t++) r[t] = piece(BM + wr + t * 16 + (lane & 15));
 #pragma unroll
             for (int v = 0; v < QT; v++) q[v] = piece(wq + v * 16 + (lane & 15));
-            if (h == 0 && step + STAGES - 1 < steps) fill();        // behind the first LDS reads: these are waited for, the fill is not
+            if (h == 0 && step + 1 < steps) fill();        // behind the first LDS reads: these are waited for, the fill is not
 #pragma unroll
             for (int w = 0; w < 2; w++) {
                 v8b rb[RT];
@@ -223,8 +221,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void scores_tile_kernel(const uint8_
                 }
             }
         }
-        stage = stage + 1 == STAGES ? 0 : stage + 1;
-        stored++;
+        stage ^= 1;
         if (++b == nb) {
             const int64_t m0 = (int64_t)(tile % m_tiles) * BM, n0 = (int64_t)(tile / m_tiles) * BN;
             const int64_t q0 = m0 + wq + (lane >> 4) * 4, j = n0 + wr + (lane & 15) * 4;
@@ -239,7 +236,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void scores_tile_kernel(const uint8_
                         for (int t = 0; t < 4; t++) o[t] = (T)acc[t][v][i];
                         __builtin_memcpy(to + (v * 16 + i) * ld, o, sizeof(o));
                     }
-                stored = 0;
+                stored = true;
             } else {
 #pragma unroll
                 for (int v = 0; v < QT; v++)
@@ -258,12 +255,12 @@ __global__ __launch_bounds__(WAVES * 64, 2) void scores_tile_kernel(const uint8_
     }
 }
 
-template <class T, int QT, int WQ, int WAVES, int STAGES>
+template <class T, int QT, int WQ, int WAVES>
 void launch_tiles(hipStream_t s, const uint8_t* qc, const uint8_t* qs, int m, const uint8_t* rc, const uint8_t* rs, int n, int nb, int nb4, T* out, int64_t ld) {
     using Shape = TileShape<QT, WQ, WAVES>;
-    constexpr int bytes = STAGES * Shape::stage, per_cu = 8 / WAVES;      // two waves a SIMD
+    constexpr int bytes = 2 * Shape::stage, per_cu = 8 / WAVES;      // two waves a SIMD
     static_assert(bytes * per_cu <= 160 * 1024, "LDS of a CU");
-    auto kernel = scores_tile_kernel<T, QT, WQ, WAVES, STAGES>;
+    auto kernel = scores_tile_kernel<T, QT, WQ, WAVES>;
     HIP_CHECK(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
     const int mt = (int)ceil_div(m, Shape::BM), nt = (int)ceil_div(n, Shape::BN);
     const int64_t groups = std::min<int64_t>(256 * per_cu, round_up((int64_t)mt * nt, 8));
@@ -290,9 +287,9 @@ template <class T> void scores_t(hipStream_t s, const Fp8View& q, int64_t q_firs
         T* o = out + i * ld + j;
         if (mi <= kStreamQueries) launch_kernel(scores_stream_kernel<T>, ceil_div(nj, 256), 256, 0, s, qc, qs, mi, rc, rs, nj, r.nb, r.nb4, o, ld);
         else switch (pick_tile(mi, nj)) {
-            case Tile::large: launch_tiles<T, 8, 2, 8, 2>(s, qc, qs, mi, rc, rs, nj, r.nb, r.nb4, o, ld); break;
-            case Tile::middle: launch_tiles<T, 4, 2, 4, 2>(s, qc, qs, mi, rc, rs, nj, r.nb, r.nb4, o, ld); break;
-            case Tile::small: launch_tiles<T, 2, 2, 4, 2>(s, qc, qs, mi, rc, rs, nj, r.nb, r.nb4, o, ld); break;
+            case Tile::large: launch_tiles<T, 8, 2, 8>(s, qc, qs, mi, rc, rs, nj, r.nb, r.nb4, o, ld); break;
+            case Tile::middle: launch_tiles<T, 4, 2, 4>(s, qc, qs, mi, rc, rs, nj, r.nb, r.nb4, o, ld); break;
+            case Tile::small: launch_tiles<T, 2, 2, 4>(s, qc, qs, mi, rc, rs, nj, r.nb, r.nb4, o, ld); break;
         }
     }
 }
