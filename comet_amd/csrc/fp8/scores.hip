@@ -129,7 +129,9 @@ __device__ __forceinline__ void fill4(const uint8_t* address, uint32_t lds /* un
     asm volatile("s_nop 4\n\tglobal_load_lds_dword %0, off" :: "v"(address), "{m0}"(__builtin_amdgcn_readfirstlane((int)lds)) : "memory");
 }
 __device__ __forceinline__ uint32_t lds_address(const void* p) { return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)p; }
-template <int N> __device__ __forceinline__ void wait_vm() { asm volatile("s_waitcnt vmcnt(%0)" :: "n"(N) : "memory"); }
+// All but the newest N global accesses of the wave are done, and its LDS reads have returned: the barrier behind this hands the buffer they read to the other
+// waves' fills, which the compiler does not see, so it would not have to wait for them here.
+template <int N> __device__ __forceinline__ void wait_buffers() { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" :: "n"(N) : "memory"); }
 
 template <class T, int QT, int WQ, int WAVES>
 __global__ __launch_bounds__(WAVES * 64, 2) void scores_tile_kernel(const uint8_t* __restrict__ qc, const uint8_t* __restrict__ qs, int m, const uint8_t* __restrict__ rc,
@@ -188,8 +190,8 @@ __global__ __launch_bounds__(WAVES * 64, 2) void scores_tile_kernel(const uint8_
     for (int step = 0; step < steps; step++) {
         // Block `step` has arrived when nothing is left that was issued before its fill or in it: behind it came only such a tile's stores, and a tile at the
         // edge, whose number of stores differs from wave to wave, is waited for with them.
-        if (stored) wait_vm<QT * 4>();
-        else wait_vm<0>();
+        if (stored) wait_buffers<QT * 4>();
+        else wait_buffers<0>();
         stored = false;
         __builtin_amdgcn_s_barrier();       // ... for every wave, and every wave is done with the buffer that is filled next
         asm volatile("" ::: "memory");

@@ -92,3 +92,13 @@ def test_asm_names_the_registers_it_takes():
                 assert '"{m0}"' in operands, (f.name, stmt)
                 seen += 1
     assert seen
+
+
+def test_buffers_are_read_before_they_are_handed_over():
+    """in front of each bare barrier the wave waits for its LDS reads: what is filled behind the barrier is filled by asm statements that the compiler does not see"""
+    text = (Path(__file__).resolve().parent.parent / "comet_amd" / "csrc" / "fp8" / "scores.hip").read_text()
+    waits = re.findall(r"void (\w+)\(\) \{ asm volatile\(\"s_waitcnt vmcnt\(%0\) lgkmcnt\(0\)\"", text)
+    assert len(waits) == 1
+    for before in text.split("__builtin_amdgcn_s_barrier()")[:-1]:
+        lines = [line.strip() for line in before.rstrip().splitlines() if not line.strip().startswith("//")][-4:]
+        assert sum(waits[0] + "<" in line for line in lines) == 2, lines         # both branches
