@@ -36,6 +36,13 @@ def _i32(x: int, what: str) -> int:
     return x
 
 
+def _i64(x: int, what: str) -> int:
+    x = int(x)
+    if not -(1 << 63) <= x < 1 << 63:
+        raise ValueError(f"{what} {x} does not fit 64 bits")
+    return x
+
+
 def _host(a: np.ndarray):
     return a.ctypes.data_as(C.c_void_p)
 
@@ -55,7 +62,7 @@ class Fp8Rows:
     def __init__(self, ctx: Context, capacity: int, dim: int):
         self.ctx, self.lib = ctx, ctx.lib
         h = C.c_void_p()
-        check(self.lib.comet_fp8_create(ctx.h, int(capacity), _i32(dim, "dimension"), C.byref(h)))
+        check(self.lib.comet_fp8_create(ctx.h, _i64(capacity, "capacity"), _i32(dim, "dimension"), C.byref(h)))
         self.h = h
         self.capacity, self.dim = int(capacity), int(dim)
 
@@ -77,20 +84,20 @@ class Fp8Rows:
     # device arrays
     def write_dev(self, vecs: int, n: int, dtype: str = "f32", ld: int | None = None, slots: int = 0, first: int = 0, stream: int | None = None) -> None:
         """row i of ``vecs`` (n rows, ``ld`` elements apart) to slot slots[i] (device int64; outside the store: skipped), or first + i"""
-        check(self.lib.comet_fp8_write_dev(self.h, C.c_void_p(slots or None), int(first), C.c_void_p(vecs or None), _dtype(dtype), int(self.dim if ld is None else ld), int(n),
-                                           self._stream(stream)))
+        check(self.lib.comet_fp8_write_dev(self.h, C.c_void_p(slots or None), _i64(first, "first slot"), C.c_void_p(vecs or None), _dtype(dtype),
+                                           _i64(self.dim if ld is None else ld, "row stride"), _i64(n, "row count"), self._stream(stream)))
 
     def read_dev(self, out: int, n: int, dtype: str = "f32", ld: int | None = None, slots: int = 0, first: int = 0, stream: int | None = None) -> None:
         """out[i] = the row in slot slots[i] (outside the store: zeros), or first + i"""
-        check(self.lib.comet_fp8_read_dev(self.h, C.c_void_p(slots or None), int(first), C.c_void_p(out or None), _dtype(dtype), int(self.dim if ld is None else ld), int(n),
-                                          self._stream(stream)))
+        check(self.lib.comet_fp8_read_dev(self.h, C.c_void_p(slots or None), _i64(first, "first slot"), C.c_void_p(out or None), _dtype(dtype),
+                                          _i64(self.dim if ld is None else ld, "row stride"), _i64(n, "row count"), self._stream(stream)))
 
     def scores_dev(self, queries: "Fp8Rows", m: int, out: int, dtype: str = "f32", ld: int | None = None, q_first: int = 0, first: int = 0, n: int | None = None,
                    stream: int | None = None) -> None:
         """out[i][j] = <queries' slot q_first + i, this store's slot first + j>, m x n (default: all slots from ``first``)"""
         n = self.capacity - first if n is None else n
-        check(self.lib.comet_fp8_scores_dev(queries.h, int(q_first), int(m), self.h, int(first), int(n), C.c_void_p(out or None), _dtype(dtype), int(n if ld is None else ld),
-                                            self._stream(stream)))
+        check(self.lib.comet_fp8_scores_dev(queries.h, _i64(q_first, "first query"), _i64(m, "query count"), self.h, _i64(first, "first slot"), _i64(n, "row count"), C.c_void_p(out or None),
+                                            _dtype(dtype), _i64(n if ld is None else ld, "row stride"), self._stream(stream)))
 
     # host arrays
     def _slots(self, slots, n: int) -> np.ndarray:
@@ -125,7 +132,7 @@ class Fp8Rows:
         B, k = _i32(q.shape[0], "query count"), _i32(k, "k")
         kk = k if 0 <= k <= 128 else 0           # any other is refused below
         r = Fp8SearchResult(np.empty((B, kk), np.int64), np.empty((B, kk), np.float32), np.empty(B, np.float32), np.empty(B, np.float32))
-        check(self.lib.comet_fp8_search(self.h, int(first), int(n), _host(q), B, C.c_float(scale), k, _host(r.slots), _host(r.logprobs), _host(r.logsum), _host(r.entropy)))
+        check(self.lib.comet_fp8_search(self.h, _i64(first, "first slot"), _i64(n, "row count"), _host(q), B, C.c_float(scale), k, _host(r.slots), _host(r.logprobs), _host(r.logsum), _host(r.entropy)))
         return r
 
 
@@ -136,7 +143,7 @@ class LogProbs:
     def __init__(self, ctx: Context, m: int, n: int, k: int):
         self.ctx, self.lib = ctx, ctx.lib
         size = C.c_size_t()
-        check(self.lib.comet_logprobs_work_bytes(int(m), int(n), _i32(k, "k"), C.byref(size)))
+        check(self.lib.comet_logprobs_work_bytes(_i64(m, "row count"), _i64(n, "column count"), _i32(k, "k"), C.byref(size)))
         self.work_bytes = size.value
         self.work = ctx.alloc(self.work_bytes) if self.work_bytes else 0
 
@@ -156,6 +163,6 @@ class LogProbs:
                 targets: int = 0, n_targets: int = 0, out_logprobs: int = 0, k: int = 0, out_ids: int = 0, out_top_logprobs: int = 0, stream: int | None = None) -> None:
         """scores: m x n, ``ld`` elements apart; counts (m), targets (m x n_targets) and out_ids (m x k) are int32, the other outputs float32"""
         p = lambda a: C.c_void_p(a or None)  # noqa: E731
-        check(self.lib.comet_logprobs_dev(self.ctx.h, p(scores), _dtype(dtype), int(n if ld is None else ld), int(m), int(n), p(counts), C.c_float(scale), p(targets),
+        check(self.lib.comet_logprobs_dev(self.ctx.h, p(scores), _dtype(dtype), _i64(n if ld is None else ld, "row stride"), _i64(m, "row count"), _i64(n, "column count"), p(counts), C.c_float(scale), p(targets),
                                           _i32(n_targets, "target count"), _i32(k, "k"), p(out_logprobs), p(out_logsum), p(out_entropy), p(out_ids), p(out_top_logprobs), p(self.work),
                                           self.work_bytes, C.c_void_p(self.ctx.stream if stream is None else int(stream))))

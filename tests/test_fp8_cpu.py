@@ -102,3 +102,21 @@ def test_buffers_are_read_before_they_are_handed_over():
     for before in text.split("__builtin_amdgcn_s_barrier()")[:-1]:
         lines = [line.strip() for line in before.rstrip().splitlines() if not line.strip().startswith("//")][-4:]
         assert sum(waits[0] + "<" in line for line in lines) == 2, lines         # both branches
+
+
+def test_numbers_beyond_64_bits_are_refused_before_they_are_cut():
+    from types import SimpleNamespace
+
+    from comet_amd import Fp8Rows, LogProbs
+    ctx = SimpleNamespace(lib=_lib.load(), h=None, stream=0)
+    R, big = Fp8Rows.__new__(Fp8Rows), 1 << 64
+    R.ctx, R.lib, R.h, R.capacity, R.dim = ctx, ctx.lib, None, 8, 8
+    plan = LogProbs(ctx, 1, 10, 1)
+    for f in (lambda: Fp8Rows(ctx, big + 8, 8), lambda: R.write_dev(16, big + 1), lambda: R.write_dev(16, 1, first=big), lambda: R.write_dev(16, 1, ld=big + 8),
+              lambda: R.read_dev(16, big + 1), lambda: R.read_dev(16, 1, first=-big), lambda: R.read_dev(16, 1, ld=big + 8), lambda: R.scores_dev(R, big + 1, 16, n=8),
+              lambda: R.scores_dev(R, 1, 16, n=big + 8), lambda: R.scores_dev(R, 1, 16, first=big, n=8), lambda: R.scores_dev(R, 1, 16, q_first=big, n=8),
+              lambda: R.scores_dev(R, 1, 16, n=8, ld=big + 8), lambda: R.search(np.zeros(8), 1, first=big), lambda: R.search(np.zeros(8), 1, n=big + 1), lambda: LogProbs(ctx, big + 1, 10, 1),
+              lambda: LogProbs(ctx, 1, big + 10, 1), lambda: plan.run_dev(16, "f32", big + 1, 10, out_logsum=16, out_entropy=16),
+              lambda: plan.run_dev(16, "f32", 1, big + 10, out_logsum=16, out_entropy=16), lambda: plan.run_dev(16, "f32", 1, 10, ld=big + 10, out_logsum=16, out_entropy=16)):
+        with pytest.raises(ValueError, match="64 bits"):
+            f()
