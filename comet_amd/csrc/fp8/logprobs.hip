@@ -9,10 +9,13 @@
 // A key is (score, column) in 64 bits, larger is better, equal scores to the lower column; keys are unique, so the result does not depend on the order in
 // which candidates arrive. Candidates wait as the score's own bits over the column's complement and become keys when they are sorted.
 //
-// Bound by reading the scores once where rows are long: 256 x 1000000 float32 take 175 us (5.9 TB/s) without the best columns and 195 us (5.3 TB/s) with the best
-// 100; 1000 ragged rows of up to 30011 bfloat16 take 16 and, with the best 20, 26 us (a call that reads nothing takes 8): a row is eight chunks, and a chunk with
-// candidates costs its workgroup a barrier and the candidates' stores. Chunks of 16 numbers a thread: 32 took 223 us for the first, 8 177 us for 1024 x 200000
-// bfloat16 that now take 154.
+// What bounds it. Long rows of float32 without the best columns: reading the scores (256 x 1000000: 175 us, 5.9 TB/s). With the best columns, and in 16-bit types,
+// the vector instructions of a score: 256 x 1000000 take 196 us with the best 100 whether they are float32 (5.2 TB/s), bfloat16 or float16 (2.6), 1024 x 200000
+// 155 and 157; 19 vector instructions a score, the vector units busy 70 - 75 % of the time (11 without the best columns: 1024 x 200000 bfloat16 in 95 us,
+// 4.3 TB/s). 1000 ragged rows of up to 30011 bfloat16 take 16 and, with the best 20, 26 us (a call that reads nothing takes 8): one workgroup a row, so the
+// longest rows' eight chunks one after the other set the time, and a chunk with candidates costs its workgroup a barrier and the candidates' stores. Rows shorter
+// than a chunk: a workgroup each, its numbers loaded one by one (2048 x 300 float32, best 10: 19 us; 2048 x 4096, a whole chunk: 17). Chunks of 16 numbers a
+// thread: 32 took 223 us for the first, 8 177 us for 1024 x 200000 bfloat16.
 #include "fp8.hpp"
 #include "lanes.hpp"
 
@@ -23,7 +26,8 @@ constexpr int kThreads = 256, kWaves = kThreads / 64, kEpt = 16, kChunk = kThrea
 // Candidate buffer: the k best so far and one chunk's survivors. When more than kSoft would be held, the chunk is cut to the keys not below the k-th
 // largest of the 256 threads' largest keys: only the k threads above that bound hold survivors, kEpt each. (Up to k = 32 quads of threads do.)
 constexpr int kSoft = 512, kCap = kLogProbsMaxK + kEpt * kLogProbsMaxK;
-// Splits of a row: enough workgroups for four per CU. A row of up to four chunks is not split: a second launch costs more than the chunks one after the other
+// Splits of a row: as many as keep the workgroups within four per CU, so one for more than 512 rows (float32, best 10: 512 x 300000 in two splits 119 us, 600 in
+// one 137, 1024 in one 214: 5.2, 5.3 and 5.7 TB/s). A row of up to four chunks is not split: a second launch costs more than the chunks one after the other
 // (1 x 10000, k = 10: 10.6 us a pass, against 14.5 split in three).
 constexpr int64_t kGroups = 1024, kWhole = 4;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;

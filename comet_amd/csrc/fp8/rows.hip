@@ -3,8 +3,10 @@
 // A block is 128 consecutive values of a row. With A the largest finite |x| of the block, e is the least integer with A * 2^-e <= 448 (the largest
 // e4m3 number) and the codes are e4m3(x * 2^-e), rounded to nearest even: multiplying by a power of two is exact, so a code is off by half a step of
 // e4m3 and by nothing else (2^-4 of the value; 2^-10 * 2^e below 2^-6 * 2^e). Both directions move each byte once and are
-// bound by HBM: 131072 x 768 float32 are written in 120 us (4.2 TB/s; the marking launch before it 6.5 us) and read as bfloat16 in 53 us (5.7 TB/s), 25600 x 768
-// scattered rows are read as float32 in 19 us (5.1 TB/s).
+// bound by HBM where rows are wide and many: 131072 x 768 float32 are written in 122 us (4.1 TB/s; the marking launch before it 6.5 us) and read as bfloat16 in
+// 53 us (5.7 TB/s), 25600 x 768 scattered rows are read as float32 in 19 us (5.2 TB/s). Narrow rows to scattered slots are bound by accesses, not bytes: a row
+// touches `last` three times (mark, look, reset), its codes and its scale, each a line of its own (1000000 x 16 float32: marking 38 us, writing 74). A single row
+// is one group's work when it is read and one workgroup's when it is written (1 x 1048576 float32: 1.46 ms read back, 0.36 ms written).
 #include "fp8.hpp"
 #include "lanes.hpp"
 
@@ -125,7 +127,7 @@ __global__ __launch_bounds__(256) void write_kernel(const T* __restrict__ x, int
 }
 
 // Rows of at most one block: groups of L lanes, as few as hold a row's V * L numbers, take U rows each, so that short rows leave no lane idle and a workgroup
-// has 32 rows or more (1000000 x 16 float32 and back: 166 us, 1000000 x 64: 237, against 307 and 375 with a block's 32 lanes a row and 8
+// has 32 rows or more (1000000 x 16 float32 and back as float32: 166 us, 1000000 x 64: 237, against 307 and 375 with a block's 32 lanes a row and 8
 // rows a workgroup). The padding's codes are zero since the store was made.
 template <class T, int L, int DUP>
 __global__ __launch_bounds__(256) void write_short_kernel(const T* __restrict__ x, int64_t ld, int n, int dim, const int64_t* __restrict__ slots, int64_t first,
@@ -205,8 +207,10 @@ __global__ __launch_bounds__(256) void read_kernel(const uint8_t* __restrict__ c
     }
 }
 
-// Rows of at most half a block: 2^shift lanes a row, as few as hold it (1000000 x 16 float32: 48 us, against 110 with a block's lanes a row; rows of more than
-// half a block are read faster by the kernel above: 234375 x 128 bfloat16 in 22 us, against 27).
+// Rows of at most half a block: 2^shift lanes a row, as few as hold it (1000000 x 16 float32: 44 - 48 us, against 110 with a block's lanes a row). Rows of more
+// than half a block are read faster by the kernel above (234375 x 128 bfloat16 in 18 - 22 us, against 27). Part of that is how a lane stores: behind the
+// early return for col >= dim the compiler stores a lane's first number in front of store_piece's branch, so its 16 bytes leave as two (float32) or four
+// (16-bit) stores, where the kernel above has one.
 template <class T>
 __global__ __launch_bounds__(256) void read_short_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, int64_t capacity, int dim, const int64_t* __restrict__ slots,
                                                          int64_t first, T* __restrict__ out, int64_t ld, int64_t n, int shift) {
@@ -295,8 +299,11 @@ void launch_fp8_write(hipStream_t s, const Fp8View& v, int32_t* last, const int6
         else lanes(std::integral_constant<int, 32>{});
         return;
     }
-    // blocks a group: two read a bulk of rows at the rate of a copy (131072 x 768 float32 and back as bfloat16: 175 us, against 219 with one and 189 with four); rows of
-    // three blocks leave no group half empty
+    // Blocks a group takes: two, and three for rows of three. Written and read back as bfloat16, 100 million numbers in rows of 2 / 3 / 5 / 6 / 7 / 9 / 16 blocks, us:
+    //   float32   two: 197 / 196 / 186 / 174 / 176 / 187 / 179   three: 205 / 183 / 187 / 176 / 176 / 176 / 188   one: 212 / 228 / 246 / 218 / 200 / 188 / 177
+    //   bfloat16  two: 167 / 167 / 159 / 154 / 151 / 153 / 161   three: 171 / 162 / 161 / 157 / 158 / 155 / 161   one: 171 / 165 / 159 / 173 / 162 / 195 / 151
+    // Rows of 300 numbers, whose third block is short: two 271 and 234, three 219 and 200. Other odd counts leave a smaller part of their groups empty and gain
+    // nothing that both types share; four blocks were slower than two nearly everywhere (768 wide: 188 and 164).
     if (v.nb == 3) blocks(std::integral_constant<int, 3>{});
     else blocks(std::integral_constant<int, 2>{});
 }

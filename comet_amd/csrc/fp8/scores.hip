@@ -14,10 +14,13 @@
 // The order of k inside a block is free as long as both operands use the same one (a block has one scale), so lane l takes row l % 16 and the 16-byte
 // pieces l / 16 and 4 + l / 16 of its 128: every load instruction covers 64 consecutive bytes of 16 rows.
 //
-// What bounds it: one query reads the rows at 5.6 TB/s (1 x 1M x 768: 139 us). 256 x 1M x 768 in float32 (410 us) moves 1.8 GB at 4.4 TB/s, more than half of it
-// written. Long rows run at the rate of the card's matrix units under load: 2048 x 32768 x 4096 at 1.36 PFLOP/s, as fast as a library product of bfloat16 rows
-// (8192^3: 1.37 - 1.40); leaving the conversions out changes nothing there (429 us against 425), never filling a buffer again 366. 2047 x 30011 x 2000 (208 us,
-// 1.18 PFLOP/s) adds what a tile costs besides its products, about 5 us a round of the chip in which all tiles are stored at once, and 944 tiles in 3.7 rounds.
+// What bounds it: one query reads the rows at 5.6 TB/s (1 x 1M x 768: 139 us). 256 x 1M x 768 in float32 (407 - 432 us from one card to another) moves 1.8 GB
+// at 4.2 - 4.4 TB/s, more than half of it written. Long rows run at the rate of the card's matrix units under load: 2048 x 32768 x 4096 at 1.29 - 1.37 PFLOP/s,
+// as fast as a library product of bfloat16 rows (8192^3: 1.37 - 1.40); leaving the conversions out changes nothing there (429 us against 425 on one card), never
+// filling a buffer again 366. 2047 x 30011 x 2000 (206 - 220 us, 1.1 - 1.2 PFLOP/s) adds what a tile costs besides its products, about 5 us a round of the chip
+// in which all tiles are stored at once, and 944 tiles in 3.7 rounds. Small stores of long rows are bound by latency: a wave walks its 64 rows' blocks one after
+// the other (1 x 1000 x 2048: 19 us in the kernel, 32 x 1000 x 2048: 15). A row narrower than a block costs what a whole block costs, in bytes and in products
+// (1 x 1M: 22 us for 16 numbers a row as for 128; 256 x 1M x 16: 239 us, most of it the scores' 1 GB).
 // Measured and left out: the next block's fill in front of a tile's stores, behind a barrier of its own (430 us for 256 x 1M x 768, against 413), operands read
 // one step ahead with a single barrier late in a block (441), a fixed order with a conversion or two between matrix instructions (421, and registers spill for
 // 16-bit scores), conversion once a workgroup into bfloat16 LDS tiles (459), workgroups started apart so that their stores do not meet (408 - 418).
@@ -60,7 +63,8 @@ template <class T> __device__ __forceinline__ void store4(T* row, int64_t j, int
 }
 
 // Up to four queries: the stored rows stream once through the registers, each wave 64 rows against an operand of queries whose blocks come out of the caches
-// (1 x 1M x 768: 139 us, 5.6 TB/s, against 149 with the smallest tile below; 16 queries: 184 against 175).
+// (1 x 1M x 768: 139 us, 5.6 TB/s, against 149 with the smallest tile below; 16 queries: 184 against 175). Two blocks in flight or one ahead in registers
+// were no faster for 1M rows (140 and 145 us); where latency counts, in stores of few rows, they were not tried.
 constexpr int kStreamQueries = 4;
 template <class T>
 __global__ __launch_bounds__(256) void scores_stream_kernel(const uint8_t* __restrict__ qc, const uint8_t* __restrict__ qs, int m, const uint8_t* __restrict__ rc,

@@ -12,7 +12,8 @@ import (
 )
 
 // Fp8Rows is a store of rows in 8-bit floating point: `capacity` slots of `dim` numbers, quantised as they are written (e4m3 codes, a power-of-two
-// scale per block of 128 numbers: 1.01 bytes a number), searched by inner product and read back. No training; any slot can be rewritten at any time.
+// scale per block of 128 numbers: 1.02 bytes a number at 768 numbers a row, more where the last block is not full: 1.3 at 300, 2.1 at 64, 8.5 at 16),
+// searched by inner product and read back. No training; any slot can be rewritten at any time.
 // Scores are those of the quantised numbers, where the indexes of this package return the reference's exact ones: a store for candidates that are
 // rescored, or for a language model that reads the best documents of a query with their probabilities.
 type Fp8Rows struct {
@@ -105,6 +106,7 @@ func (r *Fp8Rows) Read(slots []int64) ([][]float32, error) {
 }
 
 // Search scores each query against the slots [first, first + n) and returns its k (at most 128) slots of largest scale * score as a distribution over all n.
+// Every slot of the window counts: one that was never written is a row of zeros with score 0, and a row that holds a NaN makes the statistics of every query NaN.
 func (r *Fp8Rows) Search(queries [][]float32, first, n int64, k int, scale float32) ([]Fp8Result, error) {
 	B := len(queries)
 	if B == 0 {

@@ -377,7 +377,8 @@ COMET_API int comet_index_get_stat(const comet_index* idx, const char* name, dou
 
 /* ---- rows in 8-bit floating point --------------------------------------------------------------------
  * A store of `capacity` slots, each holding one row of `dim` numbers as e4m3 codes with a power-of-two scale per block of 128 consecutive
- * numbers (the last block padded with zeros): 1.01 bytes a number instead of 4, no training, any slot rewritten at any time. The reference's
+ * numbers (the last block padded with zeros), no training, any slot rewritten at any time. A slot takes 128 bytes a block, the scales rounded up to 4
+ * bytes, and 4 bytes for writes that name it twice: 1.02 bytes a number at 768 numbers a row, 1.3 at 300, 2.1 at 64, 8.5 at 16 (float32: 4). The reference's
  * nearest relatives are the quantisers of quantizer.go, which none of its indexes uses; scores here are of quantised rows where the indexes' are exact.
  *   A = largest finite |x| of the block; e = the least integer with A * 2^-e <= 448, at least -126 (a block of zeros: -126);
  *   code = e4m3(x * 2^-e), to nearest, ties to even (off by at most 2^-4 of the value, or 2^(e-10) where that is more); value = code * 2^e, exactly.
@@ -385,8 +386,8 @@ COMET_API int comet_index_get_stat(const comet_index* idx, const char* name, dou
  * counts as infinity; in products, numbers below 2^-126 may count as 0.) A slot that was never written holds zeros.
  *
  * `*_dev` calls queue their work on `stream` (a hipStream_t of the context's device; NULL: the device's null stream; comet_ctx_stream(ctx): lane 0)
- * and return. They allocate nothing and wait for nothing, so they can be captured into a HIP graph; a graph replays the pointers and sizes of the
- * captured call. Calls on one store from several streams are the caller's to order (reads and products may overlap each other). Device arrays of any
+ * and return. They allocate nothing and wait for nothing, a call of another thread that holds the context included, so they can be captured into a HIP graph;
+ * a graph replays the pointers and sizes of the captured call. Calls on one store from several streams are the caller's to order (reads and products may overlap each other). Device arrays of any
  * stride (`ld`, in elements) and any alignment down to the element's are taken. The host-array forms run on lane 0 and return when done. */
 typedef struct comet_fp8_rows comet_fp8_rows;
 typedef enum { COMET_F32 = 0, COMET_F16 = 1, COMET_BF16 = 2 } comet_dtype;
@@ -424,7 +425,9 @@ COMET_API int comet_logprobs_dev(comet_ctx* ctx, const void* scores_dev, int dty
                                  const int32_t* targets_dev, int32_t n_targets, int32_t k, float* out_logprobs_dev, float* out_logsum_dev, float* out_entropy_dev,
                                  int32_t* out_ids_dev, float* out_top_logprobs_dev, void* work_dev, size_t work_bytes, void* stream);
 /* B queries (host, B x dim) against slots [first, first + n) of a store in one call: quantised as a write would, scored, and for each query the k slots of
- * largest scale * score with their log-probabilities among the n (B x k), logsum and entropy (B). Host arrays. */
+ * largest scale * score with their log-probabilities among the n (B x k), logsum and entropy (B). Host arrays. Every slot of the window counts: one that was
+ * never written is a row of zeros, with score 0, and one row that holds a NaN makes logsum, entropy and log p of every query NaN. There is no mask and no
+ * deletion: keep the window to what is written, or score and rank with comet_fp8_scores_dev and comet_logprobs_dev, which take masked scores and counts. */
 COMET_API int comet_fp8_search(const comet_fp8_rows* rows, int64_t first, int64_t n, const float* queries, int32_t B, float scale, int32_t k, int64_t* out_slots,
                                float* out_logprobs, float* out_logsum, float* out_entropy);
 
