@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 
 import fp8_ref as ref
-from comet_amd import Fp8Rows
+from comet_amd import Fp8Rows, LogProbs
 from test_fp8_gpu import DTYPES, Dev, check_logprobs, read, rows_of, run_logprobs, same, score_rows, scores, write
 
 pytestmark = pytest.mark.gpu
@@ -89,3 +89,87 @@ def test_search_over_slots_that_were_never_written(ctx):
     r = R.search(q, k, scale, first=21)
     assert np.isfinite(r.logsum).all() and (r.slots >= 21).all()
     R.close()
+
+
+def test_host_writes_and_reads_of_more_rows_than_one_piece(ctx):
+    """uploads of 256 MiB at a time, the same slots in two of them: the last row stays (ones and minus ones are held exactly)"""
+    dim, n = 1 << 20, 70                # 64 rows a piece
+    rng = np.random.default_rng(9)
+    x = rng.integers(0, 2, (n, dim), np.int8).astype(np.float32) * 2 - 1
+    slots = np.arange(n) % 67           # rows 67, 68 and 69 over rows 0, 1 and 2
+    R = Fp8Rows(ctx, 67, dim)
+    R.write(x, slots)
+    want = x[:67].copy()
+    want[:3] = x[67:]
+    at = np.r_[np.arange(67), [0, 66, 1]]
+    assert (R.read(at) == want[at]).all()
+    R.close()
+
+
+def test_strides_behind_32_bits(ctx):
+    """two rows 2^31 + 3 elements apart, of each matrix that the calls take"""
+    torch = pytest.importorskip("torch")
+    ld, dim, n, k = (1 << 31) + 3, 300, 5000, 10
+    x, q = rows_of(80, n, dim), rows_of(81, 2, dim)
+    st = torch.cuda.current_stream().cuda_stream
+    buf = torch.zeros(ld + n + 7, dtype=torch.bfloat16, device="cuda")
+    R, Q, plan = Fp8Rows(ctx, n, dim), Fp8Rows(ctx, 2, dim), LogProbs(ctx, 2, n, k)
+    R.write(x, np.arange(n))
+    qb = torch.from_numpy(q).to(torch.bfloat16)
+    for i in range(2):
+        buf[i * ld:i * ld + dim] = qb[i].cuda()
+    Q.write_dev(buf.data_ptr(), 2, "bf16", ld=ld, stream=st)
+    hq, h = ref.held(qb.float().numpy()), ref.held(x)
+    buf.zero_()
+    Q.read_dev(buf.data_ptr(), 2, "bf16", ld=ld, stream=st)
+    got = torch.stack([buf[:dim], buf[ld:ld + dim]]).float().cpu().numpy()
+    assert same(got, hq) and buf[dim:ld].any().item() is False       # (bfloat16 holds the values exactly)
+    R.scores_dev(Q, 2, buf.data_ptr(), "bf16", ld=ld, stream=st)
+    s = torch.stack([buf[:n], buf[ld:ld + n]]).float().cpu().numpy()
+    want, mag = hq @ h.T, np.abs(hq) @ np.abs(h).T
+    assert (np.abs(s - want) <= dim * 2.0 ** -23 * mag + ref.EPS["bf16"] * np.abs(want) * 1.01).all()
+    ls, en, tl = (torch.empty(2, *sh, device="cuda") for sh in ((), (), (k,)))
+    ids = torch.empty(2, k, dtype=torch.int32, device="cuda")
+    plan.run_dev(buf.data_ptr(), "bf16", 2, n, ld=ld, scale=5.0, out_logsum=ls.data_ptr(), out_entropy=en.data_ptr(), k=k, out_ids=ids.data_ptr(), out_top_logprobs=tl.data_ptr(), stream=st)
+    check_logprobs({"ids": ids.cpu().numpy(), "top": tl.cpu().numpy(), "logsum": ls.cpu().numpy(), "entropy": en.cpu().numpy(), "logprobs": np.empty((2, 0), np.float32)}, s, n, None, 5.0, None, k)
+    for p in (R, Q, plan):
+        p.close()
+
+
+def test_the_longest_score_row(ctx):
+    """2^30 columns: all of score 0 but one at the front and the last"""
+    torch = pytest.importorskip("torch")
+    n, k = 1 << 30, 4
+    st = torch.cuda.current_stream().cuda_stream
+    s = torch.zeros(n, dtype=torch.float16, device="cuda")
+    s[12345], s[n - 1] = 2.0, 3.0
+    plan = LogProbs(ctx, 1, n, k)
+    ls, en, tl, lp = (torch.empty(i, device="cuda") for i in (1, 1, k, 3))
+    ids, targets = torch.empty(k, dtype=torch.int32, device="cuda"), torch.tensor([n - 1, 12345, n - 2], dtype=torch.int32, device="cuda")
+    plan.run_dev(s.data_ptr(), "f16", 1, n, scale=4.0, targets=targets.data_ptr(), n_targets=3, out_logprobs=lp.data_ptr(), out_logsum=ls.data_ptr(), out_entropy=en.data_ptr(), k=k,
+                 out_ids=ids.data_ptr(), out_top_logprobs=tl.data_ptr(), stream=st)
+    z = np.array([12.0, 8.0, 0.0])
+    logsum = np.log(np.exp(z) @ np.array([1.0, 1.0, n - 2.0]))
+    p = np.exp(z - logsum)
+    # a thread adds up whole numbers (exp(0) times the columns), the larger terms are joined with a rounding each: some tens of steps of 2^-24 in S, and those of z and log S
+    tol = 64 * 2.0 ** -23 * (1 + abs(logsum))
+    assert ids.tolist() == [n - 1, 12345, 0, 1]
+    assert abs(ls.item() - logsum) <= tol and abs(en.item() + (p * (z - logsum)) @ np.array([1.0, 1.0, n - 2.0])) <= tol
+    assert np.abs(tl.cpu().numpy() - (z - logsum)[[0, 1, 2, 2]]).max() <= tol and np.abs(lp.cpu().numpy() - (z - logsum)).max() <= tol
+    plan.close()
+
+
+def test_scores_of_more_than_2_31_elements(ctx, dev):
+    torch = pytest.importorskip("torch")
+    m, n, dim = 256, 8_500_001, 3
+    rng = np.random.default_rng(10)
+    q, r = rng.integers(-7, 8, (m, dim)).astype(np.float32), rng.integers(-7, 8, (n, dim)).astype(np.float32)
+    Q, R = Fp8Rows(ctx, m, dim), Fp8Rows(ctx, n, dim)
+    write(dev, Q, q); write(dev, R, r)
+    ctx.sync()
+    out = torch.zeros(m, n, dtype=torch.bfloat16, device="cuda")
+    R.scores_dev(Q, m, out.data_ptr(), "bf16", stream=torch.cuda.current_stream().cuda_stream)
+    dq, dr = torch.from_numpy(q).cuda(), torch.from_numpy(r).cuda()
+    for i in (0, 1, 252, 253, 254, 255):
+        assert torch.equal(out[i].float(), (dr @ dq[i]).to(torch.bfloat16).float()), i         # whole numbers below 2^8: exact
+    Q.close(); R.close()
